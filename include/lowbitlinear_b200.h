@@ -268,6 +268,53 @@ int lbl_w4a16_dequantize(const int32_t* packed_w, const float* scales, const int
                          void* weight, int weight_is_fp32, int64_t N, int64_t K, int group_size,
                          int device, void* stream);
 
+/* ---- Microscaled 4-bit floating point --------------------------------------------------------
+ * Formats with E2M1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign) and one scale per block of columns:
+ *   LBL_FP4_MX  blocks of 32, E8M0 scale byte: step = 2^(byte - 127)
+ *   LBL_FP4_NV  blocks of 16, E4M3 scale byte and one FP32 factor g per tensor: step = scale * g
+ * An operand [R, K] is stored as
+ *   codes   uint8 [R, 16 * ceil(K / 32)], two codes to a byte, low nibble first, zero past column K
+ *   scales  uint8 [ceil(R / 128), ceil(blocks / 4), 32, 4, 4] (blocks: of the columns padded to 32): the
+ *           byte of row r and block j is at [r / 128, j / 4, r % 32, r % 128 / 32, j % 4]
+ * Factors are pointers to one float on the device, null meaning 1; they belong to LBL_FP4_NV only
+ * (LBL_ERR_INVALID otherwise).  Codes and scales have to be 16-byte aligned, activations and outputs
+ * aligned to their type.  Rows and columns up to 2^30.  No call allocates, synchronises or retains
+ * anything; all can be captured. */
+#define LBL_FP4_MX 0
+#define LBL_FP4_NV 1
+#define LBL_TYPE_F16 0
+#define LBL_TYPE_BF16 1
+#define LBL_TYPE_F32 2
+
+/* x [rows, cols], `row_stride` elements between rows -> codes, scales.
+ *   MX: step = 2^max(floor(log2 amax) - 2, -127)   NV: scale = nearest E4M3 to amax / (6 g), at most 448
+ *   code = nearest E2M1 to x / step, ties to the even code, at most 6
+ * A block with a NaN or an infinity gets the NaN scale (0xFF, 0x7F) and zero codes; so does every block
+ * when g is not between 2^-64 and 2^64.  Padding rows and blocks of `scales` are written as zero. */
+int lbl_fp4_quantize(const void* x, int x_type, int64_t rows, int64_t cols, int64_t row_stride,
+                     int format, const float* factor, void* codes, void* scales, int device,
+                     void* stream);
+
+/* out [rows, cols] = code * step in FP32, rounded once to out_type. */
+int lbl_fp4_dequantize(const void* codes, const void* scales, int64_t rows, int64_t cols, int format,
+                       const float* factor, void* out, int out_type, int device, void* stream);
+
+/* out [M, N] (FP16 or BF16) = a [M, K] . b [N, K]^T, both quantised; FP32 sums. */
+int lbl_fp4_matmul(const void* a_codes, const void* a_scales, const float* a_factor,
+                   const void* b_codes, const void* b_scales, const float* b_factor, void* out,
+                   int64_t M, int64_t N, int64_t K, int format, int out_type, unsigned flags,
+                   int device, void* stream);
+
+/* y [M, N] = quantised x [M, K] . w [N, K]^T; x and y FP16 or BF16 (x_type), x_row_stride elements
+ * between the rows of x.  The numbers of lbl_fp4_quantize followed by lbl_fp4_matmul.  The workspace
+ * (lbl_fp4_linear_workspace_bytes, may be 0; 16-byte aligned) holds the quantised x during the call and
+ * needs no initial value; calls that overlap on the GPU need separate ones. */
+size_t lbl_fp4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int format);
+int lbl_fp4_linear(const void* x, int x_type, int64_t x_row_stride, const float* x_factor,
+                   const void* w_codes, const void* w_scales, const float* w_factor, void* y,
+                   int64_t M, int64_t N, int64_t K, int format, void* workspace,
+                   size_t workspace_bytes, unsigned flags, int device, void* stream);
+
 /* Reads (and clears) the device-side status word of `device`: 0, or a code left by a
  * kernel whose bounded wait on a barrier expired.  Synchronises the device. */
 int lbl_device_status(int device, int* status);

@@ -6,5 +6,6 @@ exported class.  ``tensor_parallel`` adds the N-split / K-split sharding helpers
 """
 from . import _extension
 from .linear import QuantizedLinear
+from .microscaling import MicroscaledLinear
 
-__all__ = ["QuantizedLinear"]
+__all__ = ["QuantizedLinear", "MicroscaledLinear"]

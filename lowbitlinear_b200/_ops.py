@@ -121,6 +121,16 @@ def bind(path):
     lib.lbl_w4a16_gemv_noalloc.argtypes = [p, p, p, p, p, i64, i64, i32, u32, i32, p]
     lib.lbl_w4a16_gemv_noalloc_scratch_bytes.restype = sz
     lib.lbl_w4a16_gemv_noalloc_scratch_bytes.argtypes = []
+    lib.lbl_fp4_quantize.restype = i32
+    lib.lbl_fp4_quantize.argtypes = [p, i32, i64, i64, i64, i32, p, p, p, i32, p]
+    lib.lbl_fp4_dequantize.restype = i32
+    lib.lbl_fp4_dequantize.argtypes = [p, p, i64, i64, i32, p, p, i32, i32, p]
+    lib.lbl_fp4_matmul.restype = i32
+    lib.lbl_fp4_matmul.argtypes = [p, p, p, p, p, p, p, i64, i64, i64, i32, i32, u32, i32, p]
+    lib.lbl_fp4_linear_workspace_bytes.restype = sz
+    lib.lbl_fp4_linear_workspace_bytes.argtypes = [i64, i64, i64, i32]
+    lib.lbl_fp4_linear.restype = i32
+    lib.lbl_fp4_linear.argtypes = [p, i32, i64, p, p, p, p, p, i64, i64, i64, i32, p, sz, u32, i32, p]
     _lib = lib
     return lib
 
@@ -502,6 +512,81 @@ def dequantize(packed_w, scales, zeros, in_features=None, dtype=torch.float16, g
                                      weight.data_ptr(), int(dtype == torch.float32), n, k, group_size,
                                      packed_w.device.index, stream))
     return weight
+
+
+FP4_FORMATS = {"mxfp4": 0, "nvfp4": 1}
+FP4_TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+
+
+def _fp4_library():
+    if _lib is None:
+        from ._extension import load_cuda_extension
+
+        load_cuda_extension(required=True)
+    return _lib
+
+
+def _pointer(tensor):
+    return None if tensor is None else tensor.data_ptr()
+
+
+def fp4_quantize(x, format, tensor_scale=None):
+    """Microscaled quantisation of a CUDA matrix in one kernel (``microscaling.quantize_fp4``, which
+    checks the arguments).  Rows may be strided; other layouts are made contiguous first."""
+    lib = _fp4_library()
+    if x.stride(1) != 1 or x.stride(0) < 0:
+        x = x.contiguous()
+    rows, k = x.shape
+    block = 16 if format == "nvfp4" else 32
+    columns = (k + 31) // 32 * 16
+    codes = torch.empty((rows, columns), dtype=torch.uint8, device=x.device)
+    scales = torch.empty(((rows + 127) // 128, (columns * 2 // block + 3) // 4, 32, 4, 4), dtype=torch.uint8,
+                         device=x.device)
+    _check(lib.lbl_fp4_quantize(x.data_ptr(), FP4_TYPES[x.dtype], rows, k, x.stride(0), FP4_FORMATS[format],
+                                _pointer(tensor_scale), codes.data_ptr(), scales.data_ptr(), x.device.index,
+                                _raw_stream(x.device)))
+    return codes, scales
+
+
+def fp4_dequantize(codes, scales, in_features, format, tensor_scale=None, dtype=torch.float16):
+    """The inverse (``microscaling.dequantize_fp4``)."""
+    lib = _fp4_library()
+    rows = codes.size(0)
+    out = torch.empty((rows, in_features), dtype=dtype, device=codes.device)
+    _check(lib.lbl_fp4_dequantize(codes.data_ptr(), scales.data_ptr(), rows, in_features, FP4_FORMATS[format],
+                                  _pointer(tensor_scale), out.data_ptr(), FP4_TYPES[dtype], codes.device.index,
+                                  _raw_stream(codes.device)))
+    return out
+
+
+def fp4_matmul(a_codes, a_scales, b_codes, b_scales, format, a_scale=None, b_scale=None, dtype=torch.float16):
+    """Product of two quantised operands (``microscaling.matmul_fp4``)."""
+    lib = _fp4_library()
+    m, n, k = a_codes.size(0), b_codes.size(0), a_codes.size(1) * 2
+    out = torch.empty((m, n), dtype=dtype, device=a_codes.device)
+    _check(lib.lbl_fp4_matmul(a_codes.data_ptr(), a_scales.data_ptr(), _pointer(a_scale), b_codes.data_ptr(),
+                              b_scales.data_ptr(), _pointer(b_scale), out.data_ptr(), m, n, k, FP4_FORMATS[format],
+                              FP4_TYPES[dtype], _flags, a_codes.device.index, _raw_stream(a_codes.device)))
+    return out
+
+
+def fp4_linear(x, codes, scales, format, tensor_scale=None, input_scale=None):
+    """Linear layer with quantised weights and activations (``microscaling.linear_fp4``).  The scratch
+    for the quantised activations is allocated per call, so calls on different streams, and graphs
+    captured from them, share nothing."""
+    lib = _fp4_library()
+    if x.stride(1) != 1 or x.stride(0) < 0:
+        x = x.contiguous()
+    m, k = x.shape
+    n = codes.size(0)
+    kind = FP4_FORMATS[format]
+    y = torch.empty((m, n), dtype=x.dtype, device=x.device)
+    need = lib.lbl_fp4_linear_workspace_bytes(m, n, k, kind)
+    scratch = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    _check(lib.lbl_fp4_linear(x.data_ptr(), FP4_TYPES[x.dtype], x.stride(0), _pointer(input_scale), codes.data_ptr(),
+                              scales.data_ptr(), _pointer(tensor_scale), y.data_ptr(), m, n, k, kind,
+                              _pointer(scratch), need, _flags, x.device.index, _raw_stream(x.device)))
+    return y
 
 
 def select_path(m, n, k, op=1):

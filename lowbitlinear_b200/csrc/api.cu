@@ -425,6 +425,155 @@ int lbl_w4a16_dequantize(const int32_t* packed_w, const float* scales, const int
   return LBL_OK;
 }
 
+// ---- microscaled FP4 -----------------------------------------------------------------------
+}  // extern "C"
+
+namespace {
+
+constexpr int64_t kFp4MaxDim = 1LL << 30;
+
+int check_fp4_shape(int64_t a, int64_t b, int64_t K, int format, const float* fa, const float* fb) {
+  if (format != LBL_FP4_MX && format != LBL_FP4_NV) return fail(LBL_ERR_INVALID, "unknown FP4 format %d", format);
+  if (a < 0 || b < 0 || K <= 0 || a > kFp4MaxDim || b > kFp4MaxDim || K > kFp4MaxDim) {
+    return fail(LBL_ERR_INVALID, "Invalid FP4 shape (%lld, %lld, K=%lld)", (long long)a, (long long)b, (long long)K);
+  }
+  if (format == LBL_FP4_MX && (fa != nullptr || fb != nullptr)) {
+    return fail(LBL_ERR_INVALID, "a tensor factor belongs to the NV format only");
+  }
+  return LBL_OK;
+}
+
+bool aligned_to(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+size_t fp4_code_bytes(int64_t rows, int64_t K) { return static_cast<size_t>(rows) * ((K + 31) / 32 * 16); }
+size_t fp4_scale_bytes(int64_t rows, int64_t K, int format) {
+  const int64_t tile_cols = format == LBL_FP4_NV ? 64 : 128;
+  const int64_t padded = (K + 31) / 32 * 32;
+  return static_cast<size_t>((rows + 127) / 128) * ((padded + tile_cols - 1) / tile_cols) * 512;
+}
+
+int run_fp4_matmul(const lbl::Fp4Operand& a, const lbl::Fp4Operand& b, int64_t K, int format, void* out, int out_type,
+                   cudaStream_t stream, const DeviceInfo& info) {
+  const cudaError_t err = lbl::launch_fp4_gemm(a, b, format, out, out_type, K, info.status_word, stream);
+  if (err != cudaSuccess) return fail_cuda(err, "FP4 product launch");
+  return LBL_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int lbl_fp4_quantize(const void* x, int x_type, int64_t rows, int64_t cols, int64_t row_stride, int format,
+                     const float* factor, void* codes, void* scales, int device, void* stream) {
+  int rc = check_fp4_shape(rows, 0, cols, format, factor, nullptr);
+  if (rc != LBL_OK) return rc;
+  if (x_type != LBL_TYPE_F16 && x_type != LBL_TYPE_BF16 && x_type != LBL_TYPE_F32) {
+    return fail(LBL_ERR_INVALID, "unknown type %d", x_type);
+  }
+  if (row_stride < 0) return fail(LBL_ERR_INVALID, "negative row stride");
+  if (rows == 0) return LBL_OK;
+  if (x == nullptr || codes == nullptr || scales == nullptr) return fail(LBL_ERR_INVALID, "null tensor pointer");
+  if (!aligned16(codes) || !aligned16(scales) || !aligned_to(x, x_type == LBL_TYPE_F32 ? 4 : 2) || !aligned_to(factor, 4)) {
+    return fail(LBL_ERR_INVALID, "codes and scales must be 16-byte aligned, x and the factor to their type");
+  }
+  DeviceScope scope(device);
+  if (!scope.ok()) return fail(LBL_ERR_CUDA, "cannot make device %d current", device);
+  const cudaError_t err =
+      lbl::launch_fp4_quantize(x, x_type, row_stride, format, factor, static_cast<uint8_t*>(codes),
+                               static_cast<uint8_t*>(scales), rows, cols, static_cast<cudaStream_t>(stream));
+  if (err != cudaSuccess) return fail_cuda(err, "FP4 quantise launch");
+  return LBL_OK;
+}
+
+int lbl_fp4_dequantize(const void* codes, const void* scales, int64_t rows, int64_t cols, int format,
+                       const float* factor, void* out, int out_type, int device, void* stream) {
+  int rc = check_fp4_shape(rows, 0, cols, format, factor, nullptr);
+  if (rc != LBL_OK) return rc;
+  if (out_type != LBL_TYPE_F16 && out_type != LBL_TYPE_BF16 && out_type != LBL_TYPE_F32) {
+    return fail(LBL_ERR_INVALID, "unknown type %d", out_type);
+  }
+  if (rows == 0) return LBL_OK;
+  if (codes == nullptr || scales == nullptr || out == nullptr) return fail(LBL_ERR_INVALID, "null tensor pointer");
+  if (!aligned16(codes) || !aligned16(scales) || !aligned_to(out, out_type == LBL_TYPE_F32 ? 4 : 2) || !aligned_to(factor, 4)) {
+    return fail(LBL_ERR_INVALID, "codes and scales must be 16-byte aligned, out and the factor to their type");
+  }
+  DeviceScope scope(device);
+  if (!scope.ok()) return fail(LBL_ERR_CUDA, "cannot make device %d current", device);
+  const cudaError_t err =
+      lbl::launch_fp4_dequantize(static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), format, factor,
+                                 out, out_type, rows, cols, static_cast<cudaStream_t>(stream));
+  if (err != cudaSuccess) return fail_cuda(err, "FP4 dequantise launch");
+  return LBL_OK;
+}
+
+int lbl_fp4_matmul(const void* a_codes, const void* a_scales, const float* a_factor, const void* b_codes,
+                   const void* b_scales, const float* b_factor, void* out, int64_t M, int64_t N, int64_t K, int format,
+                   int out_type, unsigned flags, int device, void* stream) {
+  (void)flags;
+  int rc = check_fp4_shape(M, N, K, format, a_factor, b_factor);
+  if (rc != LBL_OK) return rc;
+  if (out_type != LBL_TYPE_F16 && out_type != LBL_TYPE_BF16) return fail(LBL_ERR_INVALID, "out must be FP16 or BF16");
+  if (M == 0 || N == 0) return LBL_OK;
+  if (a_codes == nullptr || a_scales == nullptr || b_codes == nullptr || b_scales == nullptr || out == nullptr) {
+    return fail(LBL_ERR_INVALID, "null tensor pointer");
+  }
+  if (!aligned16(a_codes) || !aligned16(a_scales) || !aligned16(b_codes) || !aligned16(b_scales) ||
+      !aligned_to(out, 2) || !aligned_to(a_factor, 4) || !aligned_to(b_factor, 4)) {
+    return fail(LBL_ERR_INVALID, "codes and scales must be 16-byte aligned, out and the factors to their type");
+  }
+  DeviceScope scope(device);
+  if (!scope.ok()) return fail(LBL_ERR_CUDA, "cannot make device %d current", device);
+  DeviceInfo info;
+  rc = device_info(device, &info);
+  if (rc != LBL_OK) return rc;
+  const lbl::Fp4Operand a = {static_cast<const uint8_t*>(a_codes), static_cast<const uint8_t*>(a_scales), a_factor, M};
+  const lbl::Fp4Operand b = {static_cast<const uint8_t*>(b_codes), static_cast<const uint8_t*>(b_scales), b_factor, N};
+  return run_fp4_matmul(a, b, K, format, out, out_type, static_cast<cudaStream_t>(stream), info);
+}
+
+size_t lbl_fp4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int format) {
+  if (M <= 0 || N <= 0 || K <= 0 || (format != LBL_FP4_MX && format != LBL_FP4_NV)) return 0;
+  return fp4_code_bytes(M, K) + fp4_scale_bytes(M, K, format);
+}
+
+int lbl_fp4_linear(const void* x, int x_type, int64_t x_row_stride, const float* x_factor, const void* w_codes,
+                   const void* w_scales, const float* w_factor, void* y, int64_t M, int64_t N, int64_t K, int format,
+                   void* workspace, size_t workspace_bytes, unsigned flags, int device, void* stream) {
+  (void)flags;
+  int rc = check_fp4_shape(M, N, K, format, x_factor, w_factor);
+  if (rc != LBL_OK) return rc;
+  if (x_type != LBL_TYPE_F16 && x_type != LBL_TYPE_BF16) return fail(LBL_ERR_INVALID, "x must be FP16 or BF16");
+  if (x_row_stride < 0) return fail(LBL_ERR_INVALID, "negative row stride");
+  if (M == 0 || N == 0) return LBL_OK;
+  if (x == nullptr || w_codes == nullptr || w_scales == nullptr || y == nullptr) {
+    return fail(LBL_ERR_INVALID, "null tensor pointer");
+  }
+  if (!aligned16(w_codes) || !aligned16(w_scales) || !aligned_to(x, 2) || !aligned_to(y, 2) || !aligned_to(x_factor, 4) ||
+      !aligned_to(w_factor, 4)) {
+    return fail(LBL_ERR_INVALID, "codes and scales must be 16-byte aligned, x, y and the factors to their type");
+  }
+  const size_t need = lbl_fp4_linear_workspace_bytes(M, N, K, format);
+  if (need > 0) {
+    if (workspace == nullptr || workspace_bytes < need) {
+      return fail(LBL_ERR_WORKSPACE, "FP4 linear needs %zu bytes of scratch, got %zu", need, workspace_bytes);
+    }
+    if (!aligned16(workspace)) return fail(LBL_ERR_INVALID, "workspace must be 16-byte aligned");
+  }
+  DeviceScope scope(device);
+  if (!scope.ok()) return fail(LBL_ERR_CUDA, "cannot make device %d current", device);
+  DeviceInfo info;
+  rc = device_info(device, &info);
+  if (rc != LBL_OK) return rc;
+  const cudaStream_t cu_stream = static_cast<cudaStream_t>(stream);
+  uint8_t* codes = static_cast<uint8_t*>(workspace);
+  uint8_t* scales = codes + fp4_code_bytes(M, K);  // a multiple of 16 bytes
+  const cudaError_t err = lbl::launch_fp4_quantize(x, x_type, x_row_stride, format, x_factor, codes, scales, M, K, cu_stream);
+  if (err != cudaSuccess) return fail_cuda(err, "FP4 quantise launch");
+  const lbl::Fp4Operand a = {codes, scales, x_factor, M};
+  const lbl::Fp4Operand b = {static_cast<const uint8_t*>(w_codes), static_cast<const uint8_t*>(w_scales), w_factor, N};
+  return run_fp4_matmul(a, b, K, format, y, x_type, cu_stream, info);
+}
+
 int lbl_device_status(int device, int* status) {
   if (status == nullptr) return fail(LBL_ERR_INVALID, "status is null");
   DeviceScope scope(device);

@@ -169,4 +169,24 @@ size_t gemm_wt_workspace_bytes(int64_t M, int64_t N, int64_t K, int sm_count);
 cudaError_t launch_gemm_wt(const Problem& p, int* status_word, cudaStream_t stream, void* workspace,
                            size_t workspace_bytes, int sm_count, bool pdl);
 
+// ----- microscaled FP4 (fp4_quantize.cu, fp4_gemm.cu) --------------------------------------------
+constexpr int kTypeF16 = 0;
+constexpr int kTypeBf16 = 1;
+constexpr int kTypeF32 = 2;
+// x [rows, cols] with `row_stride` elements between rows -> codes [rows, 16 ceil(cols / 32)], tiled scales
+// (padding rows and blocks written as zero).  factor: FP32 tensor factor of NVFP4 on the device, null = 1.
+cudaError_t launch_fp4_quantize(const void* x, int x_type, int64_t row_stride, int format, const float* factor,
+                                uint8_t* codes, uint8_t* scales, int64_t rows, int64_t cols, cudaStream_t stream);
+cudaError_t launch_fp4_dequantize(const uint8_t* codes, const uint8_t* scales, int format, const float* factor,
+                                  void* out, int out_type, int64_t rows, int64_t cols, cudaStream_t stream);
+struct Fp4Operand {
+  const uint8_t* codes;
+  const uint8_t* scales;
+  const float* factor;  // null = 1
+  int64_t rows;
+};
+// out [a.rows, b.rows] = a . b^T, FP16 or BF16; K >= 1, rows >= 1, every buffer 16-byte aligned.
+cudaError_t launch_fp4_gemm(const Fp4Operand& a, const Fp4Operand& b, int format, void* out, int out_type, int64_t K,
+                            int* status_word, cudaStream_t stream);
+
 }  // namespace lbl
