@@ -23,7 +23,7 @@ except ImportError:  # run as a plain script
 
 OUTPUT = PACKAGE_DIR / "_C.so"
 SOURCES = ("api.cu", "generic.cu", "skinny.cu", "gemv_decode.cu", "gemv_grouped.cu", "peer_reduce.cu", "gemm_tc.cu", "gemm_tc2.cu", "gemm_tc_small.cu", "gemm_wt.cu", "quantize.cu",
-           "fp4_quantize.cu", "fp4_gemm.cu", "tensor_map.cu")
+           "fp4_quantize.cu", "fp4_stream.cu", "fp4_pair.cu", "tensor_map.cu")
 ARCH_FLAGS = ("-gencode", "arch=compute_100a,code=sm_100a")
 COMMON_FLAGS = ("-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xptxas", "-v")
 

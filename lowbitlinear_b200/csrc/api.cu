@@ -452,9 +452,18 @@ size_t fp4_scale_bytes(int64_t rows, int64_t K, int format) {
   return static_cast<size_t>((rows + 127) / 128) * ((padded + tile_cols - 1) / tile_cols) * 512;
 }
 
+// Which product kernel: the pair kernel's 256 x 256 tiles when there are enough of them to fill the SMs.
+bool fp4_use_pair(int64_t M, int64_t N, int sm_count) {
+  const int64_t tiles = ((M + 255) / 256) * ((N + 255) / 256);
+  return M > 128 && 4 * tiles >= sm_count;
+}
+
 int run_fp4_matmul(const lbl::Fp4Operand& a, const lbl::Fp4Operand& b, int64_t K, int format, void* out, int out_type,
-                   cudaStream_t stream, const DeviceInfo& info) {
-  const cudaError_t err = lbl::launch_fp4_gemm(a, b, format, out, out_type, K, info.status_word, stream);
+                   bool pdl, cudaStream_t stream, const DeviceInfo& info) {
+  const cudaError_t err =
+      fp4_use_pair(a.rows, b.rows, info.sm_count)
+          ? lbl::launch_fp4_pair(a, b, format, out, out_type, K, info.sm_count, info.status_word, pdl, stream)
+          : lbl::launch_fp4_stream(a, b, format, out, out_type, K, info.sm_count, info.status_word, pdl, stream);
   if (err != cudaSuccess) return fail_cuda(err, "FP4 product launch");
   return LBL_OK;
 }
@@ -509,7 +518,6 @@ int lbl_fp4_dequantize(const void* codes, const void* scales, int64_t rows, int6
 int lbl_fp4_matmul(const void* a_codes, const void* a_scales, const float* a_factor, const void* b_codes,
                    const void* b_scales, const float* b_factor, void* out, int64_t M, int64_t N, int64_t K, int format,
                    int out_type, unsigned flags, int device, void* stream) {
-  (void)flags;
   int rc = check_fp4_shape(M, N, K, format, a_factor, b_factor);
   if (rc != LBL_OK) return rc;
   if (out_type != LBL_TYPE_F16 && out_type != LBL_TYPE_BF16) return fail(LBL_ERR_INVALID, "out must be FP16 or BF16");
@@ -528,18 +536,18 @@ int lbl_fp4_matmul(const void* a_codes, const void* a_scales, const float* a_fac
   if (rc != LBL_OK) return rc;
   const lbl::Fp4Operand a = {static_cast<const uint8_t*>(a_codes), static_cast<const uint8_t*>(a_scales), a_factor, M};
   const lbl::Fp4Operand b = {static_cast<const uint8_t*>(b_codes), static_cast<const uint8_t*>(b_scales), b_factor, N};
-  return run_fp4_matmul(a, b, K, format, out, out_type, static_cast<cudaStream_t>(stream), info);
+  return run_fp4_matmul(a, b, K, format, out, out_type, (flags & LBL_FLAG_PDL) != 0, static_cast<cudaStream_t>(stream), info);
 }
 
 size_t lbl_fp4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int format) {
   if (M <= 0 || N <= 0 || K <= 0 || (format != LBL_FP4_MX && format != LBL_FP4_NV)) return 0;
+  if (lbl::fp4_fused_supports(M, K, format)) return 0;
   return fp4_code_bytes(M, K) + fp4_scale_bytes(M, K, format);
 }
 
 int lbl_fp4_linear(const void* x, int x_type, int64_t x_row_stride, const float* x_factor, const void* w_codes,
                    const void* w_scales, const float* w_factor, void* y, int64_t M, int64_t N, int64_t K, int format,
                    void* workspace, size_t workspace_bytes, unsigned flags, int device, void* stream) {
-  (void)flags;
   int rc = check_fp4_shape(M, N, K, format, x_factor, w_factor);
   if (rc != LBL_OK) return rc;
   if (x_type != LBL_TYPE_F16 && x_type != LBL_TYPE_BF16) return fail(LBL_ERR_INVALID, "x must be FP16 or BF16");
@@ -565,13 +573,20 @@ int lbl_fp4_linear(const void* x, int x_type, int64_t x_row_stride, const float*
   rc = device_info(device, &info);
   if (rc != LBL_OK) return rc;
   const cudaStream_t cu_stream = static_cast<cudaStream_t>(stream);
+  const lbl::Fp4Operand b = {static_cast<const uint8_t*>(w_codes), static_cast<const uint8_t*>(w_scales), w_factor, N};
+  if (need == 0) {
+    const cudaError_t err = lbl::launch_fp4_fused_linear(x, x_type, x_row_stride, M, x_factor, b, format, y, K, info.sm_count,
+                                                         info.status_word, (flags & LBL_FLAG_PDL) != 0, cu_stream);
+    if (err != cudaSuccess) return fail_cuda(err, "FP4 linear launch");
+    return LBL_OK;
+  }
   uint8_t* codes = static_cast<uint8_t*>(workspace);
   uint8_t* scales = codes + fp4_code_bytes(M, K);  // a multiple of 16 bytes
   const cudaError_t err = lbl::launch_fp4_quantize(x, x_type, x_row_stride, format, x_factor, codes, scales, M, K, cu_stream);
   if (err != cudaSuccess) return fail_cuda(err, "FP4 quantise launch");
   const lbl::Fp4Operand a = {codes, scales, x_factor, M};
-  const lbl::Fp4Operand b = {static_cast<const uint8_t*>(w_codes), static_cast<const uint8_t*>(w_scales), w_factor, N};
-  return run_fp4_matmul(a, b, K, format, y, x_type, cu_stream, info);
+  // The product starts beside the quantiser and waits for it before it touches the codes.
+  return run_fp4_matmul(a, b, K, format, y, x_type, /*pdl=*/true, cu_stream, info);
 }
 
 int lbl_device_status(int device, int* status) {

@@ -1,0 +1,407 @@
+// Product of two microscaled FP4 operands, many rows on both sides: persistent kernel on pairs of CTAs.
+//
+//   out[i, j] = T( ga gb sum_k a[i, k] b[j, k] )
+//
+// Bound by the tensor pipe (a pair's MMA of 256 x 256 x 64 takes 128 cycles at the FP4 rate) and by the L2,
+// which has to deliver 64 bytes per cycle and SM at that rate with 256 x 256 tiles.  A cluster of two CTAs owns a
+// tile: each loads its 128 rows of a and its half of the 256 rows of b, tcgen05.mma.cta_group::2 reads both
+// halves of b, and each CTA accumulates its 128 rows x 256 columns.
+//
+//   warp 0      copies of both operands' codes (TMA) and scale tiles (bulk); every CTA needs the scales of all
+//               256 rows of b
+//   warp 1      first CTA: scales to tensor memory (both CTAs') and MMAs; second CTA: reports its finished copies
+//               to the first with one remote arrival per stage
+//   warps 2-5   epilogue
+//
+// Tensor memory holds two accumulators of 256 columns that overlap, [0, 256) and [208, 464), beside the 48 columns
+// of scales.  The epilogue reads the shared columns of a tile first and gives them back at once; the next
+// tile's MMAs start then and run beside the rest of the epilogue.
+#include "fp4_tc.cuh"
+
+namespace lbl {
+namespace {
+
+constexpr int kRowsCta = 128;   // rows of a, and of b, that one CTA loads
+constexpr int kRowsPair = 256;
+constexpr int kEpilogueWarps = 4;
+constexpr int kThreads = 32 * (2 + kEpilogueWarps);
+constexpr int kMaxStages = 6;
+constexpr int kStatusPairWait = 620;
+constexpr int kTmemColumns = 512;
+constexpr int kScaleColumn = 512 - 48;
+constexpr int kSecondAccumulator = kScaleColumn - kRowsPair;  // 208
+constexpr int kChunk = 64;  // columns an epilogue warp handles at a time
+constexpr int kStagingBytes = 32 * kChunk * 2;  // per epilogue warp
+constexpr int kSmemLimit = 227 * 1024;
+constexpr int kGroupRows = 8;  // row tiles that are walked together, for reuse in the L2
+
+struct PairParams {
+  const uint8_t* sf_a;
+  const uint8_t* sf_b;
+  const float* factor_a;
+  const float* factor_b;
+  void* out;
+  int64_t out_pitch;
+  int rows_a, rows_b;
+  int cols_padded;
+  int scale_tiles;  // along K
+  int tiles_a, tiles_b;
+  int vector_ok;  // 16-byte stores of out allowed
+  int* status;
+};
+
+struct PairBarriers {
+  uint64_t full[kMaxStages];   // this CTA's copies have landed
+  uint64_t empty[kMaxStages];  // the MMAs have read the stage (cluster-wide commit)
+  uint64_t peer_full[kMaxStages];  // first CTA's: the second CTA's copies have landed
+  uint64_t acc_full;               // a tile's accumulators are complete (cluster-wide commit)
+  uint64_t acc_free;               // first CTA's: both CTAs have read the shared columns
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+template <int kFormat>
+struct PairTile {
+  static constexpr int kTiles = kStageCols / fp4::Format<kFormat>::kTileCols;
+  static constexpr int kBytesCodes = kRowsCta * kRowBytes;      // of one operand
+  static constexpr int kBytesScaleA = kTiles * 512;
+  static constexpr int kBytesScaleB = 2 * kTiles * 512;
+  static constexpr int kStageBytes = 2 * kBytesCodes + kBytesScaleA + kBytesScaleB;
+  static constexpr int kStages = (kSmemLimit - 2048 - kEpilogueWarps * kStagingBytes) / kStageBytes < kMaxStages
+                                     ? (kSmemLimit - 2048 - kEpilogueWarps * kStagingBytes) / kStageBytes
+                                     : kMaxStages;
+  static constexpr int kSmemBytes = kStages * kStageBytes + kEpilogueWarps * kStagingBytes + 1024;
+  static_assert(kTiles * 4 * 3 <= 48, "scale columns");
+};
+
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t* smem_result, uint32_t cols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(smem_result)),
+               "r"(cols)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_relinquish_pair() {
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t cols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
+}
+// Arrives on the barrier at this shared-memory offset in both CTAs of the pair once every MMA
+// issued so far has finished.
+__device__ __forceinline__ void mma_commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_addr(bar)),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
+__device__ __forceinline__ void arrive_remote(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// Bounded wait with acquire semantics at cluster scope (the other CTA's arrivals order its work).
+__device__ __forceinline__ bool wait_cluster_bounded(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                                                     int* status_word, int status_code) {
+  const long long start = clock64();
+  while (true) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(smem_addr(bar)), "r"(parity)
+        : "memory");
+    if (done) return true;
+    if (*abort_flag) return false;
+    if (clock64() - start > kWaitLimitCycles) {
+      *abort_flag = 1;
+      atomicCAS(status_word, 0, status_code);
+      return false;
+    }
+  }
+}
+
+// Tile t: groups of kGroupRows row tiles, walked column by column.
+__device__ __forceinline__ void tile_of(const PairParams& p, int t, int* tile_a, int* tile_b) {
+  const int per_group = kGroupRows * p.tiles_b;
+  const int group = t / per_group;
+  const int first = group * kGroupRows;
+  const int rows = min(kGroupRows, p.tiles_a - first);
+  const int rest = t - group * per_group;
+  *tile_a = first + rest % rows;
+  *tile_b = rest / rows;
+}
+
+template <int kFormat, typename T>
+__global__ void __launch_bounds__(kThreads, 1)
+    fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                    const PairParams p) {
+  using Tile = PairTile<kFormat>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint8_t* smem_a = smem;
+  uint8_t* smem_b = smem_a + Tile::kStages * Tile::kBytesCodes;
+  uint8_t* smem_sa = smem_b + Tile::kStages * Tile::kBytesCodes;
+  uint8_t* smem_sb = smem_sa + Tile::kStages * Tile::kBytesScaleA;
+  uint8_t* staging = smem_sb + Tile::kStages * Tile::kBytesScaleB;
+  __shared__ PairBarriers bars;
+  volatile int* abort_flag = &bars.abort_flag;
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();  // 0: issues the MMAs
+  const int first_tile = blockIdx.x >> 1;
+  const int tile_step = gridDim.x >> 1;
+  const int tiles = p.tiles_a * p.tiles_b;
+  const int k_stages = (p.cols_padded + kStageCols - 1) / kStageCols;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < Tile::kStages; ++s) {
+      mbar_init(&bars.full[s], 1);
+      mbar_init(&bars.empty[s], 1);
+      mbar_init(&bars.peer_full[s], 1);
+    }
+    mbar_init(&bars.acc_full, 1);
+    mbar_init(&bars.acc_free, 2 * kEpilogueWarps);
+    bars.abort_flag = 0;
+    mbar_init_fence();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(&bars.tmem_base, kTmemColumns);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  // Both CTAs' barriers exist and both allocations are done before anybody signals across.
+  cluster_sync_all();
+  tc_fence_after_sync();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&bars.tmem_base);
+  pdl_allow_next_kernel();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      pdl_wait_for_previous_kernel();
+      int i = 0;  // stages since the start
+      for (int t = first_tile; t < tiles; t += tile_step) {
+        int tile_a, tile_b;
+        tile_of(p, t, &tile_a, &tile_b);
+        const int row_a = tile_a * kRowsPair + static_cast<int>(rank) * kRowsCta;
+        const int row_b = tile_b * kRowsPair;
+        const bool has_a = row_a < p.rows_a;
+        const int blocks_b = row_b + kRowsCta < p.rows_b ? 2 : 1;
+        for (int kb = 0; kb < k_stages; ++kb, ++i) {
+          const int s = i % Tile::kStages;
+          const int round = i / Tile::kStages;
+          if (round > 0) mbar_wait_bounded(&bars.empty[s], (round - 1) & 1, abort_flag, p.status, kStatusPairWait + 1);
+          if (*abort_flag) break;
+          const int tile0 = kb * Tile::kTiles;
+          const uint32_t bytes = min(Tile::kTiles, p.scale_tiles - tile0) * 512;
+          mbar_arrive_expect_tx(&bars.full[s], 2 * Tile::kBytesCodes + bytes * ((has_a ? 1 : 0) + blocks_b));
+          tma_load_2d(smem_a + s * Tile::kBytesCodes, &map_a, kb * kRowBytes, row_a, &bars.full[s]);
+          tma_load_2d(smem_b + s * Tile::kBytesCodes, &map_b, kb * kRowBytes, row_b + static_cast<int>(rank) * kRowsCta,
+                      &bars.full[s]);
+          // A CTA past the last row of a has no scales to load; what lies in its stage reaches rows nobody stores.
+          if (has_a) {
+            bulk_load(smem_sa + s * Tile::kBytesScaleA,
+                      p.sf_a + (static_cast<int64_t>(row_a / 128) * p.scale_tiles + tile0) * 512, bytes, &bars.full[s]);
+          }
+          for (int b = 0; b < blocks_b; ++b) {
+            bulk_load(smem_sb + s * Tile::kBytesScaleB + b * Tile::kTiles * 512,
+                      p.sf_b + (static_cast<int64_t>(row_b / 128 + b) * p.scale_tiles + tile0) * 512, bytes, &bars.full[s]);
+          }
+        }
+        if (*abort_flag) break;
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 1) {
+      const uint32_t peer_full = map_to_cta(smem_addr(&bars.peer_full[0]), 0);
+      int i = 0;
+      for (int t = first_tile; t < tiles; t += tile_step) {
+        for (int kb = 0; kb < k_stages; ++kb, ++i) {
+          const int s = i % Tile::kStages;
+          mbar_wait_bounded(&bars.full[s], (i / Tile::kStages) & 1, abort_flag, p.status, kStatusPairWait + 2);
+          if (*abort_flag) break;
+          arrive_remote(peer_full + 8u * static_cast<uint32_t>(s));
+        }
+        if (*abort_flag) break;
+      }
+    }
+    if (lane == 0 && rank == 0) {
+      int i = 0, n = 0;
+      for (int t = first_tile; t < tiles; t += tile_step, ++n) {
+        // Tile n may use its accumulator once the epilogue has read the shared columns of tile n - 1 (and with
+        // them, in program order, all of tile n - 2).
+        if (n > 0) wait_cluster_bounded(&bars.acc_free, (n - 1) & 1, abort_flag, p.status, kStatusPairWait + 3);
+        if (*abort_flag) break;
+        tc_fence_after_sync();
+        const uint32_t acc = tmem + (n & 1) * kSecondAccumulator;
+        for (int kb = 0; kb < k_stages; ++kb, ++i) {
+          const int s = i % Tile::kStages;
+          const uint32_t parity = (i / Tile::kStages) & 1;
+          mbar_wait_bounded(&bars.full[s], parity, abort_flag, p.status, kStatusPairWait + 4);
+          wait_cluster_bounded(&bars.peer_full[s], parity, abort_flag, p.status, kStatusPairWait + 5);
+          if (*abort_flag) break;
+          tc_fence_after_sync();
+          issue_stage<kFormat, 2, kRowsPair, kRowsPair>(
+              acc, tmem + kScaleColumn, smem_addr(smem_a + s * Tile::kBytesCodes), smem_addr(smem_b + s * Tile::kBytesCodes),
+              smem_addr(smem_sa + s * Tile::kBytesScaleA), smem_addr(smem_sb + s * Tile::kBytesScaleB),
+              p.cols_padded - kb * kStageCols, kb == 0);
+          mma_commit_pair(&bars.empty[s]);
+        }
+        if (*abort_flag) break;
+        mma_commit_pair(&bars.acc_full);
+      }
+    }
+  } else {
+    pdl_wait_for_previous_kernel();
+    const float alpha = product_factor(p.factor_a, p.factor_b);
+    const uint32_t acc_free = map_to_cta(smem_addr(&bars.acc_free), 0);
+    const int quarter = warp & 3;
+    uint8_t* mine = staging + (warp - 2) * kStagingBytes;
+    T* out = static_cast<T*>(p.out);
+    int n = 0;
+    for (int t = first_tile; t < tiles; t += tile_step, ++n) {
+      int tile_a, tile_b;
+      tile_of(p, t, &tile_a, &tile_b);
+      const int row0 = tile_a * kRowsPair + static_cast<int>(rank) * kRowsCta + quarter * 32;
+      const int col0 = tile_b * kRowsPair;
+      if (!mbar_wait_bounded(&bars.acc_full, n & 1, abort_flag, p.status, kStatusPairWait + 6)) break;
+      tc_fence_after_sync();
+      const uint32_t acc = tmem + (n & 1) * kSecondAccumulator + (static_cast<uint32_t>(quarter * 32) << 16);
+#pragma unroll 1
+      for (int c = 0; c < kRowsPair / kChunk; ++c) {
+        // The columns shared with the other accumulator come first: the last ones of [0, 256), the first of [208, 464).
+        const int first_col = ((n & 1) ? c : kRowsPair / kChunk - 1 - c) * kChunk;
+        uint32_t v[2][32];
+        tmem_load_32cols(acc + first_col, v[0]);
+        tmem_load_32cols(acc + first_col + 32, v[1]);
+        tmem_load_wait();
+        if (c == 0) {
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) arrive_remote(acc_free);
+        }
+        // Row `lane` of the chunk: eight pieces of 16 bytes, swizzled over the banks.
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t* f = &v[i >> 2][(i & 3) * 8];
+          uint4 q;
+          q.x = two_rounded<T>(__uint_as_float(f[0]) * alpha, __uint_as_float(f[1]) * alpha);
+          q.y = two_rounded<T>(__uint_as_float(f[2]) * alpha, __uint_as_float(f[3]) * alpha);
+          q.z = two_rounded<T>(__uint_as_float(f[4]) * alpha, __uint_as_float(f[5]) * alpha);
+          q.w = two_rounded<T>(__uint_as_float(f[6]) * alpha, __uint_as_float(f[7]) * alpha);
+          *reinterpret_cast<uint4*>(mine + lane * 128 + ((i ^ (lane & 7)) << 4)) = q;
+        }
+        __syncwarp();
+        const int piece = lane & 7;
+        const int col = col0 + first_col + piece * 8;
+#pragma unroll
+        for (int r = lane >> 3; r < 32; r += 4) {
+          const uint4 q = *reinterpret_cast<const uint4*>(mine + r * 128 + ((piece ^ (r & 7)) << 4));
+          const int row = row0 + r;
+          if (row < p.rows_a && col < p.rows_b) {
+            T* dst = out + row * p.out_pitch + col;
+            if (p.vector_ok && col + 8 <= p.rows_b) {
+              *reinterpret_cast<uint4*>(dst) = q;
+            } else {
+              const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                if (col + e < p.rows_b) {
+                  reinterpret_cast<unsigned short*>(dst)[e] = static_cast<unsigned short>(w[e >> 1] >> (16 * (e & 1)));
+                }
+              }
+            }
+          }
+        }
+        __syncwarp();
+      }
+    }
+  }
+
+  if (*abort_flag) {
+    // Give copies that are still in flight time to land before the shared memory is released.
+    const long long start = clock64();
+    while (clock64() - start < 200000) {
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  // Neither CTA may leave (or free tensor memory) while the other could still signal it.
+  cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc_pair(tmem, kTmemColumns);
+  }
+}
+
+template <int kFormat, typename T>
+cudaError_t launch(const Fp4Operand& a, const Fp4Operand& b, void* out, int64_t K, int sm_count, int* status, bool pdl,
+                   cudaStream_t stream) {
+  using Tile = PairTile<kFormat>;
+  const int64_t pitch = fp4::code_pitch(K);
+  CUtensorMap map_a, map_b;
+  if (!encode_codes(&map_a, a.codes, a.rows, pitch, kRowsCta) || !encode_codes(&map_b, b.codes, b.rows, pitch, kRowsCta)) {
+    return cudaErrorInvalidValue;
+  }
+  PairParams params;
+  params.sf_a = a.scales;
+  params.sf_b = b.scales;
+  params.factor_a = a.factor;
+  params.factor_b = b.factor;
+  params.out = out;
+  params.out_pitch = b.rows;
+  params.rows_a = static_cast<int>(a.rows);
+  params.rows_b = static_cast<int>(b.rows);
+  params.cols_padded = static_cast<int>(fp4::padded_cols(K));
+  params.scale_tiles = static_cast<int>(fp4::scale_tiles(K, kFormat));
+  const int64_t tiles_a = (a.rows + kRowsPair - 1) / kRowsPair;
+  const int64_t tiles_b = (b.rows + kRowsPair - 1) / kRowsPair;
+  if (tiles_a * tiles_b > 0x3fffffffLL) return cudaErrorInvalidConfiguration;
+  params.tiles_a = static_cast<int>(tiles_a);
+  params.tiles_b = static_cast<int>(tiles_b);
+  params.vector_ok = b.rows % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  params.status = status;
+
+  auto kernel = fp4_pair_kernel<kFormat, T>;
+  static bool configured[64] = {};
+  int device = 0;
+  cudaError_t err = cudaGetDevice(&device);
+  if (err != cudaSuccess) return err;
+  if (device < 0 || device >= 64 || !configured[device]) {
+    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile::kSmemBytes);
+    if (err != cudaSuccess) return err;
+    if (device >= 0 && device < 64) configured[device] = true;
+  }
+  const int64_t slots = sm_count >= 2 ? sm_count / 2 : 1;
+  const int64_t pairs = tiles_a * tiles_b < slots ? tiles_a * tiles_b : slots;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Tile::kSmemBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, map_a, map_b, params);
+}
+
+}  // namespace
+
+cudaError_t launch_fp4_pair(const Fp4Operand& a, const Fp4Operand& b, int format, void* out, int out_type, int64_t K,
+                            int sm_count, int* status_word, bool pdl, cudaStream_t stream) {
+  if (format == fp4::kNv) {
+    return out_type == kTypeBf16 ? launch<fp4::kNv, __nv_bfloat16>(a, b, out, K, sm_count, status_word, pdl, stream)
+                                 : launch<fp4::kNv, __half>(a, b, out, K, sm_count, status_word, pdl, stream);
+  }
+  return out_type == kTypeBf16 ? launch<fp4::kMx, __nv_bfloat16>(a, b, out, K, sm_count, status_word, pdl, stream)
+                               : launch<fp4::kMx, __half>(a, b, out, K, sm_count, status_word, pdl, stream);
+}
+
+}  // namespace lbl

@@ -23,6 +23,7 @@ __global__ void __launch_bounds__(kThreads)
     fp4_quantize_kernel(const T* __restrict__ x, int64_t row_stride, const float* __restrict__ factor,
                         uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int64_t rows, int64_t cols,
                         int units, bool vector_ok) {
+  pdl_allow_next_kernel();
   const int lane = threadIdx.x & 31;
   const int64_t row = static_cast<int64_t>(blockIdx.y) * blockDim.y + threadIdx.y;
   const int unit = blockIdx.x * blockDim.x + threadIdx.x;  // blockDim.x is a multiple of 32: a warp has one row

@@ -1,0 +1,441 @@
+// Product of a microscaled FP4 weight with few rows of activations: y[q, p] = sum_k x[q, k] w[p, k].
+//
+// Bound by the weight's bytes, so the weight takes the M side of the MMA (128 rows per CTA, streamed once
+// through a ring of TMA stages) and the activations its N side (kQ = 16 .. 256 of them).  K is cut into
+// as many slices as fill the SMs; the CTAs of one row block's slices form a cluster, leave their FP32
+// partial tiles in shared memory and add them in slice order through distributed shared memory: no
+// scratch, no atomics, the same bits every time.
+//
+//   kFused (kQ <= 32): the activations come in 16 bits and every CTA quantises its slice of them into shared
+//   memory while its first weight stages are on their way (the rounding of fp4_common.cuh), one launch
+//   for the whole linear layer.  Otherwise both operands are codes and tiled scales.
+//
+//   warp 0      copies: codes by TMA (rows of 128 bytes, 128-byte swizzle), scale tiles by bulk copies
+//   warp 1      scales to tensor memory, MMAs
+//   the others  quantisation (kFused), epilogue
+#include "fp4_tc.cuh"
+
+namespace lbl {
+namespace {
+
+constexpr int kP = 128;
+constexpr int kMaxStages = 8;
+constexpr int kMaxSplit = 8;
+constexpr int kStatusStreamWait = 600;
+
+struct StreamParams {
+  const uint8_t* sf_p;
+  const uint8_t* sf_q;
+  const float* factor_p;
+  const float* factor_q;
+  const void* x;  // kFused: 16-bit activations
+  int64_t x_stride;
+  void* out;
+  int64_t out_pitch;
+  int rows_p, rows_q;
+  int cols;         // K
+  int cols_padded;  // to 32
+  int scale_tiles;  // along K
+  int stages;
+  int split;        // CTAs of a cluster
+  int x_vector;     // 16-byte loads of x allowed
+  int* status;
+};
+
+struct StreamBarriers {
+  uint64_t full[kMaxStages];
+  uint64_t empty[kMaxStages];
+  uint64_t x_ready;
+  uint64_t done;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+template <int kFormat, int kQ, bool kFused>
+struct StreamTile {
+  static constexpr int kTiles = kStageCols / fp4::Format<kFormat>::kTileCols;
+  static constexpr int kQBlocks = (kQ + 127) / 128;
+  static constexpr int kBytesP = kP * kRowBytes;
+  static constexpr int kBytesQ = kQ * kRowBytes;
+  static constexpr int kBytesScaleP = kTiles * 512;
+  static constexpr int kBytesScaleQ = kTiles * 512 * kQBlocks;
+  static constexpr int kStageBytes = kBytesP + kBytesScaleP + (kFused ? 0 : kBytesQ + kBytesScaleQ);
+  static constexpr int kPartialBytes = kP * kQ * 4;
+  static constexpr int kColumns = kQ + kTiles * 4 * (1 + kQBlocks);
+  static constexpr int kTmemColumns = kColumns <= 64 ? 64 : kColumns <= 128 ? 128 : kColumns <= 256 ? 256 : 512;
+  static constexpr int kWorkers = kFused ? 8 : 4;  // warps
+  static constexpr int kThreads = 32 * (2 + kWorkers);
+};
+
+// Rounds this CTA's slice of the activations: sixteen columns of a row per thread and step, stage by
+// stage, into the swizzled code tiles and the scale tiles the MMAs read.  Rows past rows_q are left as
+// they are: they only reach columns of the accumulator that nobody reads.
+template <int kFormat, int kQ, typename T>
+__device__ __forceinline__ void quantise_slice(const StreamParams& p, int k_begin, int stages_here, uint8_t* codes,
+                                               uint8_t* scales, int worker, int workers) {
+  using Tile = StreamTile<kFormat, kQ, true>;
+  const fp4::TensorFactor factor = fp4::tensor_factor(kFormat == fp4::kNv ? p.factor_q : nullptr);
+  const int per_stage = p.rows_q * 16;  // even: both halves of an MXFP4 block are in one warp
+  const int total = stages_here * per_stage;
+  const int rounds = (total + workers - 1) / workers;
+  for (int i = 0; i < rounds; ++i) {
+    const int item = i * workers + worker;
+    const bool have = item < total;
+    const int stage = have ? item / per_stage : 0;
+    const int rest = item - stage * per_stage;
+    const int row = have ? rest >> 4 : 0;
+    const int unit = rest & 15;
+    const int col = (k_begin + stage) * kStageCols + unit * 16;
+    const int valid = have ? min(16, max(0, p.cols - col)) : 0;
+    const T* src = static_cast<const T*>(p.x) + row * p.x_stride + col;
+    fp4::Sixteen<T> v;
+    if (valid == 16 && p.x_vector) {
+      v.load_vector(src);
+    } else {
+      v.load_masked(src, valid);
+    }
+    uint32_t amax = v.amax_bits();
+    fp4::BlockStep step;
+    if constexpr (kFormat == fp4::kMx) {
+      amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      step = fp4::mx_step(amax);
+    } else {
+      step = fp4::nv_step(amax, factor);
+    }
+    float part[8];
+    uint2 out;
+    v.eight(0, part);
+    out.x = fp4::round_eight<kFormat, true>(part, step);
+    v.eight(1, part);
+    out.y = fp4::round_eight<kFormat, true>(part, step);
+    if (have) {
+      const uint32_t chunk = unit >> 1;
+      uint8_t* dst = codes + stage * Tile::kBytesQ + (row >> 3) * 1024 + (row & 7) * 128 +
+                     ((chunk ^ (row & 7)) << 4) + (unit & 1) * 8;
+      *reinterpret_cast<uint2*>(dst) = out;
+      const int block = kFormat == fp4::kMx ? unit >> 1 : unit;
+      scales[stage * Tile::kBytesScaleQ + (block >> 2) * 512 + row * 16 + (block & 3)] = static_cast<uint8_t>(step.byte);
+    }
+  }
+}
+
+template <int kFormat, int kQ, bool kFused, typename T>
+__global__ void __launch_bounds__(StreamTile<kFormat, kQ, kFused>::kThreads, 1)
+    fp4_stream_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
+                      const StreamParams p) {
+  using Tile = StreamTile<kFormat, kQ, kFused>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  __shared__ StreamBarriers bars;
+  volatile int* abort_flag = &bars.abort_flag;
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = p.split > 1 ? cluster_rank() : 0;
+  const int p0 = (blockIdx.x / p.split) * kP;
+  const int q0 = blockIdx.y * kQ;
+  const int k_stages = (p.cols_padded + kStageCols - 1) / kStageCols;
+  const int k_begin = static_cast<int>(static_cast<int64_t>(k_stages) * rank / p.split);
+  const int k_end = static_cast<int>(static_cast<int64_t>(k_stages) * (rank + 1) / p.split);
+  const int stages_here = k_end - k_begin;
+
+  // Code tiles first (swizzled tiles start on 1024 bytes).  kFused: Q holds the whole slice.
+  const int q_slots = kFused ? stages_here : p.stages;
+  uint8_t* smem_p = smem;
+  uint8_t* smem_q = smem_p + p.stages * Tile::kBytesP;
+  uint8_t* smem_sp = smem_q + q_slots * Tile::kBytesQ;
+  uint8_t* smem_sq = smem_sp + p.stages * Tile::kBytesScaleP;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(&bars.full[s], 1);
+      mbar_init(&bars.empty[s], 1);
+    }
+    mbar_init(&bars.x_ready, Tile::kWorkers);
+    mbar_init(&bars.done, 1);
+    bars.abort_flag = 0;
+    mbar_init_fence();
+  }
+  if (warp == 1) {
+    tmem_alloc(&bars.tmem_base, Tile::kTmemColumns);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&bars.tmem_base);
+  pdl_allow_next_kernel();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int blocks_q = 0;
+      for (int b = 0; b < Tile::kQBlocks; ++b) blocks_q += q0 + b * 128 < p.rows_q ? 1 : 0;
+      // The activations may come from the kernel in front of this one, the weight does not (a call's
+      // own quantiser is that kernel): the first stages of the weight are fetched before waiting.
+      auto load_q = [&](int i) {
+        const int kb = k_begin + i;
+        const int s = i % p.stages;
+        const int tile0 = kb * Tile::kTiles;
+        const uint32_t bytes = min(Tile::kTiles, p.scale_tiles - tile0) * 512;
+        tma_load_2d(smem_q + s * Tile::kBytesQ, &map_q, kb * kRowBytes, q0, &bars.full[s]);
+        for (int b = 0; b < blocks_q; ++b) {
+          bulk_load(smem_sq + s * Tile::kBytesScaleQ + b * Tile::kTiles * 512,
+                    p.sf_q + (static_cast<int64_t>(q0 / 128 + b) * p.scale_tiles + tile0) * 512, bytes, &bars.full[s]);
+        }
+      };
+      auto load_p = [&](int i) {
+        const int kb = k_begin + i;
+        const int s = i % p.stages;
+        const int tile0 = kb * Tile::kTiles;
+        const uint32_t bytes = min(Tile::kTiles, p.scale_tiles - tile0) * 512;
+        mbar_arrive_expect_tx(&bars.full[s], Tile::kBytesP + bytes + (kFused ? 0 : Tile::kBytesQ + bytes * blocks_q));
+        tma_load_2d(smem_p + s * Tile::kBytesP, &map_p, kb * kRowBytes, p0, &bars.full[s]);
+        bulk_load(smem_sp + s * Tile::kBytesScaleP,
+                  p.sf_p + (static_cast<int64_t>(p0 / 128) * p.scale_tiles + tile0) * 512, bytes, &bars.full[s]);
+      };
+      const int ahead = min(p.stages, stages_here);
+      for (int i = 0; i < ahead; ++i) load_p(i);
+      if constexpr (!kFused) {
+        pdl_wait_for_previous_kernel();
+        for (int i = 0; i < ahead; ++i) load_q(i);
+      }
+      for (int i = ahead; i < stages_here; ++i) {
+        mbar_wait_bounded(&bars.empty[i % p.stages], (i / p.stages - 1) & 1, abort_flag, p.status, kStatusStreamWait + 1);
+        if (*abort_flag) break;
+        load_p(i);
+        if constexpr (!kFused) load_q(i);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      if constexpr (kFused) {
+        mbar_wait_bounded(&bars.x_ready, 0, abort_flag, p.status, kStatusStreamWait + 4);
+      }
+      for (int i = 0; i < stages_here; ++i) {
+        const int s = i % p.stages;
+        mbar_wait_bounded(&bars.full[s], (i / p.stages) & 1, abort_flag, p.status, kStatusStreamWait + 2);
+        if (*abort_flag) break;
+        tc_fence_after_sync();
+        const int sq = kFused ? i : s;
+        issue_stage<kFormat, 1, kP, kQ>(tmem, tmem + kQ, smem_addr(smem_p + s * Tile::kBytesP),
+                                        smem_addr(smem_q + sq * Tile::kBytesQ), smem_addr(smem_sp + s * Tile::kBytesScaleP),
+                                        smem_addr(smem_sq + sq * Tile::kBytesScaleQ),
+                                        p.cols_padded - (k_begin + i) * kStageCols, i == 0);
+        mma_commit(&bars.empty[s]);
+      }
+      if (!*abort_flag) mma_commit(&bars.done);
+    }
+  } else {
+    pdl_wait_for_previous_kernel();
+    if constexpr (kFused) {
+      quantise_slice<kFormat, kQ, T>(p, k_begin, stages_here, smem_q, smem_sq, threadIdx.x - 64, Tile::kWorkers * 32);
+      fence_async_proxy();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.x_ready);
+    }
+    if (warp < 6) {
+      // Every MMA of the CTA is complete, so the ring's memory holds the partial tile [kQ][128] now.
+      const bool ok = mbar_wait_bounded(&bars.done, 0, abort_flag, p.status, kStatusStreamWait + 3);
+      tc_fence_after_sync();
+      if (ok) {
+        const int quarter = warp & 3;
+        const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+        float* partial = reinterpret_cast<float*>(smem) + quarter * 32 + lane;
+        const int used = min(kQ, p.rows_q - q0);
+        for (int c0 = 0; c0 < used; c0 += 32) {
+          uint32_t v[32];
+          tmem_load_32cols(taddr + c0, v);
+          tmem_load_wait();
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            if (c0 + c < kQ) partial[(c0 + c) * kP] = __uint_as_float(v[c]);
+          }
+        }
+      }
+    }
+  }
+
+  if (*abort_flag) {
+    // Give copies that are still in flight time to land before the shared memory is released.
+    const long long start = clock64();
+    while (clock64() - start < 200000) {
+    }
+  }
+  tc_fence_before_sync();
+  __syncwarp();
+  if (p.split > 1) {
+    cluster_sync_all();
+  } else {
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, Tile::kTmemColumns);
+  }
+
+  // Two neighbouring rows of the weight and one activation row per thread and step; the cluster's CTAs share
+  // the tile, and each adds the slices in their order.
+  const float alpha = product_factor(p.factor_p, p.factor_q);
+  const int used = min(kQ, p.rows_q - q0);
+  const uint32_t partial_addr = smem_addr(smem);
+  T* out = static_cast<T*>(p.out);
+  const bool paired = (p.out_pitch & 1) == 0 && (reinterpret_cast<uintptr_t>(out) & 3) == 0;
+  for (int item = rank * Tile::kThreads + threadIdx.x; item < used * (kP / 2); item += p.split * Tile::kThreads) {
+    const int q = item / (kP / 2);
+    const int row = (item % (kP / 2)) * 2;
+    const uint32_t offset = partial_addr + (q * kP + row) * 4;
+    float a = 0.0f, b = 0.0f;
+    if (p.split > 1) {
+      for (int r = 0; r < p.split; ++r) {
+        float2 v;
+        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(map_to_cta(offset, r)) : "memory");
+        a += v.x, b += v.y;
+      }
+    } else {
+      const float2 v = *reinterpret_cast<const float2*>(smem + (q * kP + row) * 4);
+      a = v.x, b = v.y;
+    }
+    if (p0 + row >= p.rows_p) continue;
+    T* dst = out + (q0 + q) * p.out_pitch + p0 + row;
+    const uint32_t y = two_rounded<T>(a * alpha, b * alpha);
+    if (paired && p0 + row + 1 < p.rows_p) {
+      *reinterpret_cast<uint32_t*>(dst) = y;
+    } else {
+      *reinterpret_cast<unsigned short*>(dst) = static_cast<unsigned short>(y & 0xFFFFu);
+      if (p0 + row + 1 < p.rows_p) *(reinterpret_cast<unsigned short*>(dst) + 1) = static_cast<unsigned short>(y >> 16);
+    }
+  }
+  // Nobody leaves while a neighbour may still read its partial tile.
+  __syncwarp();
+  if (p.split > 1) cluster_sync_all();
+}
+
+constexpr int kSmemLimit = 227 * 1024;
+constexpr int kFusedRows = 16;
+constexpr int kFusedSliceBytes = 64 * 1024;
+
+template <int kFormat, int kQ, bool kFused, typename T>
+cudaError_t launch(const Fp4Operand& w, const Fp4Operand& x, const void* raw, int64_t raw_stride, void* out, int64_t K,
+                   int sm_count, int* status, bool pdl, cudaStream_t stream) {
+  using Tile = StreamTile<kFormat, kQ, kFused>;
+  const int64_t pitch = fp4::code_pitch(K);
+  CUtensorMap map_p, map_q;
+  if (!encode_codes(&map_p, w.codes, w.rows, pitch, kP)) return cudaErrorInvalidValue;
+  if constexpr (kFused) {
+    map_q = map_p;  // not used
+  } else {
+    if (!encode_codes(&map_q, x.codes, x.rows, pitch, kQ)) return cudaErrorInvalidValue;
+  }
+  const int64_t blocks_p = (w.rows + kP - 1) / kP;
+  const int64_t blocks_q = (x.rows + kQ - 1) / kQ;
+  const int k_stages = static_cast<int>((fp4::padded_cols(K) + kStageCols - 1) / kStageCols);
+  // Slices until the SMs are busy, two stages at least in each.
+  int split = 1;
+  while (split < kMaxSplit && blocks_p * blocks_q * split * 2 <= 2 * sm_count && k_stages >= split * 4) split *= 2;
+  if constexpr (kFused) {
+    // The slice of the activations shares the memory with the ring.
+    while (split < kMaxSplit && (k_stages + split - 1) / split * (Tile::kBytesQ + Tile::kBytesScaleQ) > kFusedSliceBytes) split *= 2;
+  }
+  const int slice = (k_stages + split - 1) / split;
+
+  StreamParams params;
+  params.sf_p = w.scales;
+  params.sf_q = x.scales;
+  params.factor_p = w.factor;
+  params.factor_q = x.factor;
+  params.x = raw;
+  params.x_stride = raw_stride;
+  params.out = out;
+  params.out_pitch = w.rows;
+  params.rows_p = static_cast<int>(w.rows);
+  params.rows_q = static_cast<int>(x.rows);
+  params.cols = static_cast<int>(K);
+  params.cols_padded = static_cast<int>(fp4::padded_cols(K));
+  params.scale_tiles = static_cast<int>(fp4::scale_tiles(K, kFormat));
+  params.split = split;
+  params.x_vector = (raw_stride * 2) % 16 == 0 && reinterpret_cast<uintptr_t>(raw) % 16 == 0;
+  params.status = status;
+  const int fixed = 1024 + (kFused ? slice * (Tile::kBytesQ + Tile::kBytesScaleQ) : 0);
+  int stages = slice < 6 ? slice : 6;
+  while (stages > 1 && fixed + stages * Tile::kStageBytes > kSmemLimit - 1024) --stages;
+  params.stages = stages;
+  int smem = fixed + stages * Tile::kStageBytes;
+  if (smem < Tile::kPartialBytes + 1024) smem = Tile::kPartialBytes + 1024;
+  if (smem > kSmemLimit - 1024) return cudaErrorInvalidValue;
+
+  auto kernel = fp4_stream_kernel<kFormat, kQ, kFused, T>;
+  static bool configured[64] = {};
+  int device = 0;
+  cudaError_t err = cudaGetDevice(&device);
+  if (err != cudaSuccess) return err;
+  if (device < 0 || device >= 64 || !configured[device]) {
+    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit - 1024);
+    if (err != cudaSuccess) return err;
+    if (device >= 0 && device < 64) configured[device] = true;
+  }
+  if (blocks_q > 65535 || blocks_p * split > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks_p * split), static_cast<unsigned>(blocks_q));
+  cfg.blockDim = dim3(Tile::kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  int attrs = 0;
+  if (split > 1) {
+    attr[attrs].id = cudaLaunchAttributeClusterDimension;
+    attr[attrs].val.clusterDim.x = split;
+    attr[attrs].val.clusterDim.y = 1;
+    attr[attrs].val.clusterDim.z = 1;
+    ++attrs;
+  }
+  if (pdl) {
+    attr[attrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[attrs].val.programmaticStreamSerializationAllowed = 1;
+    ++attrs;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = attrs;
+  return cudaLaunchKernelEx(&cfg, kernel, map_p, map_q, params);
+}
+
+}  // namespace
+
+template <int kFormat, typename T>
+static cudaError_t stream_product(const Fp4Operand& a, const Fp4Operand& b, void* out, int64_t K, int sm_count,
+                                  int* status, bool pdl, cudaStream_t stream) {
+  if (a.rows <= 32) return launch<kFormat, 32, false, T>(b, a, nullptr, 0, out, K, sm_count, status, pdl, stream);
+  if (a.rows <= 64) return launch<kFormat, 64, false, T>(b, a, nullptr, 0, out, K, sm_count, status, pdl, stream);
+  return launch<kFormat, 128, false, T>(b, a, nullptr, 0, out, K, sm_count, status, pdl, stream);
+}
+
+cudaError_t launch_fp4_stream(const Fp4Operand& a, const Fp4Operand& b, int format, void* out, int out_type, int64_t K,
+                              int sm_count, int* status_word, bool pdl, cudaStream_t stream) {
+  if (format == fp4::kNv) {
+    return out_type == kTypeBf16 ? stream_product<fp4::kNv, __nv_bfloat16>(a, b, out, K, sm_count, status_word, pdl, stream)
+                                 : stream_product<fp4::kNv, __half>(a, b, out, K, sm_count, status_word, pdl, stream);
+  }
+  return out_type == kTypeBf16 ? stream_product<fp4::kMx, __nv_bfloat16>(a, b, out, K, sm_count, status_word, pdl, stream)
+                               : stream_product<fp4::kMx, __half>(a, b, out, K, sm_count, status_word, pdl, stream);
+}
+
+bool fp4_fused_supports(int64_t M, int64_t K, int format) {
+  const int64_t k_stages = (fp4::padded_cols(K) + kStageCols - 1) / kStageCols;
+  const int64_t stage_bytes = kFusedRows * kRowBytes + (format == fp4::kNv ? 4 : 2) * 512;
+  return M <= kFusedRows && (k_stages + kMaxSplit - 1) / kMaxSplit * stage_bytes <= kFusedSliceBytes;
+}
+
+cudaError_t launch_fp4_fused_linear(const void* x, int x_type, int64_t x_stride, int64_t M, const float* x_factor,
+                                    const Fp4Operand& w, int format, void* out, int64_t K, int sm_count,
+                                    int* status_word, bool pdl, cudaStream_t stream) {
+  const Fp4Operand a = {nullptr, nullptr, x_factor, M};
+  if (format == fp4::kNv) {
+    return x_type == kTypeBf16
+               ? launch<fp4::kNv, kFusedRows, true, __nv_bfloat16>(w, a, x, x_stride, out, K, sm_count, status_word, pdl, stream)
+               : launch<fp4::kNv, kFusedRows, true, __half>(w, a, x, x_stride, out, K, sm_count, status_word, pdl, stream);
+  }
+  return x_type == kTypeBf16
+             ? launch<fp4::kMx, kFusedRows, true, __nv_bfloat16>(w, a, x, x_stride, out, K, sm_count, status_word, pdl, stream)
+             : launch<fp4::kMx, kFusedRows, true, __half>(w, a, x, x_stride, out, K, sm_count, status_word, pdl, stream);
+}
+
+}  // namespace lbl

@@ -185,8 +185,18 @@ struct Fp4Operand {
   const float* factor;  // null = 1
   int64_t rows;
 };
-// out [a.rows, b.rows] = a . b^T, FP16 or BF16; K >= 1, rows >= 1, every buffer 16-byte aligned.
-cudaError_t launch_fp4_gemm(const Fp4Operand& a, const Fp4Operand& b, int format, void* out, int out_type, int64_t K,
-                            int* status_word, cudaStream_t stream);
+// out [a.rows, b.rows] = a . b^T, FP16 or BF16; K >= 1, rows >= 1, codes and scales 16-byte aligned.
+// `pdl`: programmatic dependent launch; b (the weight) must not be written by the kernel in front.
+// Few rows of a (fp4_stream.cu): b is streamed once, K is cut into slices that meet in a cluster.
+cudaError_t launch_fp4_stream(const Fp4Operand& a, const Fp4Operand& b, int format, void* out, int out_type, int64_t K,
+                              int sm_count, int* status_word, bool pdl, cudaStream_t stream);
+// The same with a given as 16-bit activations x [M, K], quantised in the kernel; out has their type.
+bool fp4_fused_supports(int64_t M, int64_t K, int format);
+cudaError_t launch_fp4_fused_linear(const void* x, int x_type, int64_t x_stride, int64_t M, const float* x_factor,
+                                    const Fp4Operand& w, int format, void* out, int64_t K, int sm_count,
+                                    int* status_word, bool pdl, cudaStream_t stream);
+// Many rows of both (fp4_pair.cu): persistent 256 x 256 tiles on pairs of CTAs.
+cudaError_t launch_fp4_pair(const Fp4Operand& a, const Fp4Operand& b, int format, void* out, int out_type, int64_t K,
+                            int sm_count, int* status_word, bool pdl, cudaStream_t stream);
 
 }  // namespace lbl

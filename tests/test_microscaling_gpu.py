@@ -121,13 +121,20 @@ def test_product_matches_64_bits(cuda_ops, fmt, m, n, k):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
-@pytest.mark.parametrize("m", [1, 3, 16, 40, 200, 600])
+@pytest.mark.parametrize("m,n,k", [(1030, 2100, 320), (1537, 2048, 33), (257, 9601, 1500), (4097, 1000, 100), (2000, 4096, 2048)])
+def test_large_products_match_64_bits(cuda_ops, fmt, m, n, k):
+    """Persistent tiles: several per CTA pair, ragged edges, rows past the last one in half of a pair."""
+    test_product_matches_64_bits(cuda_ops, fmt, m, n, k)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("m", [1, 3, 16, 40, 200, 600, 3000])
 def test_rows_do_not_touch_each_other(cuda_ops, fmt, m):
     """A row whose blocks are NaN makes its own outputs NaN; an all-zero row gives zeros; every other
     row keeps its bits."""
     g = torch.Generator().manual_seed(m)
     x = torch.randn(m, 512, generator=g).half()
-    w = torch.randn(320, 512, generator=g).half()
+    w = torch.randn(1500 if m > 1000 else 320, 512, generator=g).half()
     operands = quantize_fp4(w.to(cuda_ops), fmt)
     clean = linear_fp4(x.to(cuda_ops), *operands, fmt).cpu()
     x[m // 2] = float("nan")
@@ -136,7 +143,7 @@ def test_rows_do_not_touch_each_other(cuda_ops, fmt, m):
     w[7, 100] = float("inf")
     got = linear_fp4(x.to(cuda_ops), *quantize_fp4(w.to(cuda_ops), fmt), fmt).cpu()
     assert torch.isnan(got[m // 2]).all() and torch.isnan(got[:, 7]).all()
-    keep = torch.ones(m, 320, dtype=torch.bool)
+    keep = torch.ones(m, w.size(0), dtype=torch.bool)
     keep[m // 2], keep[:, 7] = False, False
     if m > 2:
         assert (got[0, :7] == 0).all() and (got[0, 8:] == 0).all()
