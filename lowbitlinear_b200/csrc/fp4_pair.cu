@@ -7,10 +7,9 @@
 // tile: each loads its 128 rows of a and its half of the 256 rows of b, tcgen05.mma.cta_group::2 reads both
 // halves of b, and each CTA accumulates its 128 rows x 256 columns.
 //
-//   warp 0      copies of both operands' codes (TMA) and scale tiles (bulk); every CTA needs the scales of all
-//               256 rows of b
-//   warp 1      first CTA: scales to tensor memory (both CTAs') and MMAs; second CTA: reports its finished copies
-//               to the first with one remote arrival per stage
+//   warp 0      copies of both operands' codes and scale tiles by TMA; every CTA needs the scales of all 256 rows of
+//               b.  Both CTAs' copies complete on the first CTA's barrier (the cta_group::2 form of the copy)
+//   warp 1      first CTA: scales to tensor memory (both CTAs') and MMAs
 //   warps 2-5   epilogue
 //
 // Tensor memory holds two accumulators of 256 columns that overlap, [0, 256) and [208, 464), beside the 48 columns
@@ -36,26 +35,22 @@ constexpr int kSmemLimit = 227 * 1024;
 constexpr int kGroupRows = 8;  // row tiles that are walked together, for reuse in the L2
 
 struct PairParams {
-  const uint8_t* sf_a;
-  const uint8_t* sf_b;
   const float* factor_a;
   const float* factor_b;
   void* out;
   int64_t out_pitch;
   int rows_a, rows_b;
   int cols_padded;
-  int scale_tiles;  // along K
   int tiles_a, tiles_b;
   int vector_ok;  // 16-byte stores of out allowed
   int* status;
 };
 
 struct PairBarriers {
-  uint64_t full[kMaxStages];   // this CTA's copies have landed
+  uint64_t full[kMaxStages];   // first CTA's: both CTAs' copies have landed
   uint64_t empty[kMaxStages];  // the MMAs have read the stage (cluster-wide commit)
-  uint64_t peer_full[kMaxStages];  // first CTA's: the second CTA's copies have landed
-  uint64_t acc_full;               // a tile's accumulators are complete (cluster-wide commit)
-  uint64_t acc_free;               // first CTA's: both CTAs have read the shared columns
+  uint64_t acc_full;           // a tile's accumulators are complete (cluster-wide commit)
+  uint64_t acc_free;           // first CTA's: both CTAs have read the shared columns
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -94,32 +89,18 @@ __device__ __forceinline__ void mma_commit_pair(uint64_t* bar) {
       "h"(static_cast<uint16_t>(3))
       : "memory");
 }
+// Tiled load into this CTA's shared memory that completes on a barrier of the pair's first CTA.
+__device__ __forceinline__ void tma_load_2d_pair(void* smem_dst, const CUtensorMap* map, int c0, int c1,
+                                                 uint32_t cluster_bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3}], [%4];" ::"r"(smem_addr(smem_dst)),
+      "l"(map), "r"(c0), "r"(c1), "r"(cluster_bar)
+      : "memory");
+}
 __device__ __forceinline__ void arrive_remote(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
-// Bounded wait with acquire semantics at cluster scope (the other CTA's arrivals order its work).
-__device__ __forceinline__ bool wait_cluster_bounded(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
-                                                     int* status_word, int status_code) {
-  const long long start = clock64();
-  while (true) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(smem_addr(bar)), "r"(parity)
-        : "memory");
-    if (done) return true;
-    if (*abort_flag) return false;
-    if (clock64() - start > kWaitLimitCycles) {
-      *abort_flag = 1;
-      atomicCAS(status_word, 0, status_code);
-      return false;
-    }
-  }
-}
-
 // Tile t: groups of kGroupRows row tiles, walked column by column.
 __device__ __forceinline__ void tile_of(const PairParams& p, int t, int* tile_a, int* tile_b) {
   const int per_group = kGroupRows * p.tiles_b;
@@ -134,6 +115,7 @@ __device__ __forceinline__ void tile_of(const PairParams& p, int t, int* tile_a,
 template <int kFormat, typename T>
 __global__ void __launch_bounds__(kThreads, 1)
     fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                    const __grid_constant__ CUtensorMap map_sa, const __grid_constant__ CUtensorMap map_sb,
                     const PairParams p) {
   using Tile = PairTile<kFormat>;
   extern __shared__ uint8_t smem_raw[];
@@ -146,7 +128,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* staging = smem_sb + Tile::kStages * Tile::kBytesScaleB;
   __shared__ PairBarriers bars;
   volatile int* abort_flag = &bars.abort_flag;
-  const int warp = threadIdx.x >> 5;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const int lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();  // 0: issues the MMAs
   const int first_tile = blockIdx.x >> 1;
@@ -158,7 +140,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int s = 0; s < Tile::kStages; ++s) {
       mbar_init(&bars.full[s], 1);
       mbar_init(&bars.empty[s], 1);
-      mbar_init(&bars.peer_full[s], 1);
     }
     mbar_init(&bars.acc_full, 1);
     mbar_init(&bars.acc_free, 2 * kEpilogueWarps);
@@ -178,78 +159,59 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_allow_next_kernel();
 
   if (warp == 0) {
-    if (lane == 0) {
-      pdl_wait_for_previous_kernel();
-      int i = 0;  // stages since the start
-      for (int t = first_tile; t < tiles; t += tile_step) {
-        int tile_a, tile_b;
-        tile_of(p, t, &tile_a, &tile_b);
-        const int row_a = tile_a * kRowsPair + static_cast<int>(rank) * kRowsCta;
-        const int row_b = tile_b * kRowsPair;
-        const bool has_a = row_a < p.rows_a;
-        const int blocks_b = row_b + kRowsCta < p.rows_b ? 2 : 1;
-        for (int kb = 0; kb < k_stages; ++kb, ++i) {
-          const int s = i % Tile::kStages;
-          const int round = i / Tile::kStages;
-          if (round > 0) mbar_wait_bounded(&bars.empty[s], (round - 1) & 1, abort_flag, p.status, kStatusPairWait + 1);
-          if (*abort_flag) break;
-          const int tile0 = kb * Tile::kTiles;
-          const uint32_t bytes = min(Tile::kTiles, p.scale_tiles - tile0) * 512;
-          mbar_arrive_expect_tx(&bars.full[s], 2 * Tile::kBytesCodes + bytes * ((has_a ? 1 : 0) + blocks_b));
-          tma_load_2d(smem_a + s * Tile::kBytesCodes, &map_a, kb * kRowBytes, row_a, &bars.full[s]);
-          tma_load_2d(smem_b + s * Tile::kBytesCodes, &map_b, kb * kRowBytes, row_b + static_cast<int>(rank) * kRowsCta,
-                      &bars.full[s]);
-          // A CTA past the last row of a has no scales to load; what lies in its stage reaches rows nobody stores.
-          if (has_a) {
-            bulk_load(smem_sa + s * Tile::kBytesScaleA,
-                      p.sf_a + (static_cast<int64_t>(row_a / 128) * p.scale_tiles + tile0) * 512, bytes, &bars.full[s]);
-          }
-          for (int b = 0; b < blocks_b; ++b) {
-            bulk_load(smem_sb + s * Tile::kBytesScaleB + b * Tile::kTiles * 512,
-                      p.sf_b + (static_cast<int64_t>(row_b / 128 + b) * p.scale_tiles + tile0) * 512, bytes, &bars.full[s]);
-          }
+    pdl_wait_for_previous_kernel();
+    const uint32_t full = map_to_cta(smem_addr(&bars.full[0]), 0);
+    int i = 0;  // stages since the start
+    for (int t = first_tile; t < tiles; t += tile_step) {
+      int tile_a, tile_b;
+      tile_of(p, t, &tile_a, &tile_b);
+      // Rows and scale tiles past the end of an operand read as zeros.
+      const int row_a = tile_a * kRowsPair + static_cast<int>(rank) * kRowsCta;
+      const int row_b = tile_b * kRowsPair + static_cast<int>(rank) * kRowsCta;
+      bool ok = true;
+      for (int kb = 0; kb < k_stages; ++kb, ++i) {
+        const int s = i % Tile::kStages;
+        const int round = i / Tile::kStages;
+        ok = round == 0 || warp_wait(&bars.empty[s], (round - 1) & 1, abort_flag, p.status, kStatusPairWait + 1);
+        if (!ok) break;
+        if (elect_one()) {
+          if (rank == 0) mbar_arrive_expect_tx(&bars.full[s], 2 * Tile::kStageBytes);
+          const uint32_t bar = full + 8u * static_cast<uint32_t>(s);
+          tma_load_2d_pair(smem_a + s * Tile::kBytesCodes, &map_a, kb * kRowBytes, row_a, bar);
+          tma_load_2d_pair(smem_b + s * Tile::kBytesCodes, &map_b, kb * kRowBytes, row_b, bar);
+          tma_load_2d_pair(smem_sa + s * Tile::kBytesScaleA, &map_sa, kb * Tile::kBytesScaleA / 8, row_a / 128, bar);
+          tma_load_2d_pair(smem_sb + s * Tile::kBytesScaleB, &map_sb, kb * Tile::kBytesScaleA / 8, tile_b * 2, bar);
         }
-        if (*abort_flag) break;
+        __syncwarp();
       }
+      if (!ok) break;
     }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 1) {
-      const uint32_t peer_full = map_to_cta(smem_addr(&bars.peer_full[0]), 0);
-      int i = 0;
-      for (int t = first_tile; t < tiles; t += tile_step) {
-        for (int kb = 0; kb < k_stages; ++kb, ++i) {
-          const int s = i % Tile::kStages;
-          mbar_wait_bounded(&bars.full[s], (i / Tile::kStages) & 1, abort_flag, p.status, kStatusPairWait + 2);
-          if (*abort_flag) break;
-          arrive_remote(peer_full + 8u * static_cast<uint32_t>(s));
-        }
-        if (*abort_flag) break;
-      }
-    }
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       int i = 0, n = 0;
       for (int t = first_tile; t < tiles; t += tile_step, ++n) {
         // Tile n may use its accumulator once the epilogue has read the shared columns of tile n - 1 (and with
         // them, in program order, all of tile n - 2).
-        if (n > 0) wait_cluster_bounded(&bars.acc_free, (n - 1) & 1, abort_flag, p.status, kStatusPairWait + 3);
-        if (*abort_flag) break;
+        bool ok = n == 0 || warp_wait_pair(&bars.acc_free, (n - 1) & 1, abort_flag, p.status, kStatusPairWait + 2);
+        if (!ok) break;
         tc_fence_after_sync();
         const uint32_t acc = tmem + (n & 1) * kSecondAccumulator;
         for (int kb = 0; kb < k_stages; ++kb, ++i) {
           const int s = i % Tile::kStages;
-          const uint32_t parity = (i / Tile::kStages) & 1;
-          mbar_wait_bounded(&bars.full[s], parity, abort_flag, p.status, kStatusPairWait + 4);
-          wait_cluster_bounded(&bars.peer_full[s], parity, abort_flag, p.status, kStatusPairWait + 5);
-          if (*abort_flag) break;
+          ok = warp_wait(&bars.full[s], (i / Tile::kStages) & 1, abort_flag, p.status, kStatusPairWait + 3);
+          if (!ok) break;
           tc_fence_after_sync();
-          issue_stage<kFormat, 2, kRowsPair, kRowsPair>(
-              acc, tmem + kScaleColumn, smem_addr(smem_a + s * Tile::kBytesCodes), smem_addr(smem_b + s * Tile::kBytesCodes),
-              smem_addr(smem_sa + s * Tile::kBytesScaleA), smem_addr(smem_sb + s * Tile::kBytesScaleB),
-              p.cols_padded - kb * kStageCols, kb == 0);
-          mma_commit_pair(&bars.empty[s]);
+          if (elect_one()) {
+            issue_stage<kFormat, 2, kRowsPair, kRowsPair>(
+                acc, tmem + kScaleColumn, smem_addr(smem_a + s * Tile::kBytesCodes),
+                smem_addr(smem_b + s * Tile::kBytesCodes), smem_addr(smem_sa + s * Tile::kBytesScaleA),
+                smem_addr(smem_sb + s * Tile::kBytesScaleB), p.cols_padded - kb * kStageCols, kb == 0);
+            mma_commit_pair(&bars.empty[s]);
+            if (kb == k_stages - 1) mma_commit_pair(&bars.acc_full);
+          }
+          __syncwarp();
         }
-        if (*abort_flag) break;
-        mma_commit_pair(&bars.acc_full);
+        if (!ok) break;
       }
     }
   } else {
@@ -265,7 +227,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tile_of(p, t, &tile_a, &tile_b);
       const int row0 = tile_a * kRowsPair + static_cast<int>(rank) * kRowsCta + quarter * 32;
       const int col0 = tile_b * kRowsPair;
-      if (!mbar_wait_bounded(&bars.acc_full, n & 1, abort_flag, p.status, kStatusPairWait + 6)) break;
+      if (!warp_wait(&bars.acc_full, n & 1, abort_flag, p.status, kStatusPairWait + 4)) break;
       tc_fence_after_sync();
       const uint32_t acc = tmem + (n & 1) * kSecondAccumulator + (static_cast<uint32_t>(quarter * 32) << 16);
 #pragma unroll 1
@@ -335,18 +297,28 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// Scale tiles as rows of 8-byte elements, one row per 128 rows of the operand.
+template <int kFormat>
+bool encode_scales(CUtensorMap* map, const uint8_t* scales, int64_t rows, int64_t K, int box_rows) {
+  const int64_t pitch = fp4::scale_tiles(K, kFormat) * 512;
+  const uint64_t dims[2] = {static_cast<uint64_t>(pitch / 8), static_cast<uint64_t>((rows + 127) / 128)};
+  const uint64_t strides[1] = {static_cast<uint64_t>(pitch)};
+  const uint32_t box[2] = {PairTile<kFormat>::kBytesScaleA / 8, static_cast<uint32_t>(box_rows)};
+  return encode_tensor_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT64, 2, scales, dims, strides, box,
+                           CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
 template <int kFormat, typename T>
 cudaError_t launch(const Fp4Operand& a, const Fp4Operand& b, void* out, int64_t K, int sm_count, int* status, bool pdl,
                    cudaStream_t stream) {
   using Tile = PairTile<kFormat>;
   const int64_t pitch = fp4::code_pitch(K);
-  CUtensorMap map_a, map_b;
-  if (!encode_codes(&map_a, a.codes, a.rows, pitch, kRowsCta) || !encode_codes(&map_b, b.codes, b.rows, pitch, kRowsCta)) {
+  CUtensorMap map_a, map_b, map_sa, map_sb;
+  if (!encode_codes(&map_a, a.codes, a.rows, pitch, kRowsCta) || !encode_codes(&map_b, b.codes, b.rows, pitch, kRowsCta) ||
+      !encode_scales<kFormat>(&map_sa, a.scales, a.rows, K, 1) || !encode_scales<kFormat>(&map_sb, b.scales, b.rows, K, 2)) {
     return cudaErrorInvalidValue;
   }
   PairParams params;
-  params.sf_a = a.scales;
-  params.sf_b = b.scales;
   params.factor_a = a.factor;
   params.factor_b = b.factor;
   params.out = out;
@@ -354,7 +326,6 @@ cudaError_t launch(const Fp4Operand& a, const Fp4Operand& b, void* out, int64_t 
   params.rows_a = static_cast<int>(a.rows);
   params.rows_b = static_cast<int>(b.rows);
   params.cols_padded = static_cast<int>(fp4::padded_cols(K));
-  params.scale_tiles = static_cast<int>(fp4::scale_tiles(K, kFormat));
   const int64_t tiles_a = (a.rows + kRowsPair - 1) / kRowsPair;
   const int64_t tiles_b = (b.rows + kRowsPair - 1) / kRowsPair;
   if (tiles_a * tiles_b > 0x3fffffffLL) return cudaErrorInvalidConfiguration;
@@ -389,7 +360,7 @@ cudaError_t launch(const Fp4Operand& a, const Fp4Operand& b, void* out, int64_t 
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kernel, map_a, map_b, params);
+  return cudaLaunchKernelEx(&cfg, kernel, map_a, map_b, map_sa, map_sb, params);
 }
 
 }  // namespace

@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(StreamTile<kFormat, kQ, kFused>::kThreads, 1)
                                              ~static_cast<uintptr_t>(1023));
   __shared__ StreamBarriers bars;
   volatile int* abort_flag = &bars.abort_flag;
-  const int warp = threadIdx.x >> 5;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const int lane = threadIdx.x & 31;
   const uint32_t rank = p.split > 1 ? cluster_rank() : 0;
   const int p0 = (blockIdx.x / p.split) * kP;
@@ -167,63 +167,66 @@ __global__ void __launch_bounds__(StreamTile<kFormat, kQ, kFused>::kThreads, 1)
   pdl_allow_next_kernel();
 
   if (warp == 0) {
-    if (lane == 0) {
-      int blocks_q = 0;
-      for (int b = 0; b < Tile::kQBlocks; ++b) blocks_q += q0 + b * 128 < p.rows_q ? 1 : 0;
-      // The activations may come from the kernel in front of this one, the weight does not (a call's
-      // own quantiser is that kernel): the first stages of the weight are fetched before waiting.
-      auto load_q = [&](int i) {
-        const int kb = k_begin + i;
-        const int s = i % p.stages;
-        const int tile0 = kb * Tile::kTiles;
-        const uint32_t bytes = min(Tile::kTiles, p.scale_tiles - tile0) * 512;
-        tma_load_2d(smem_q + s * Tile::kBytesQ, &map_q, kb * kRowBytes, q0, &bars.full[s]);
-        for (int b = 0; b < blocks_q; ++b) {
-          bulk_load(smem_sq + s * Tile::kBytesScaleQ + b * Tile::kTiles * 512,
-                    p.sf_q + (static_cast<int64_t>(q0 / 128 + b) * p.scale_tiles + tile0) * 512, bytes, &bars.full[s]);
-        }
-      };
-      auto load_p = [&](int i) {
-        const int kb = k_begin + i;
-        const int s = i % p.stages;
-        const int tile0 = kb * Tile::kTiles;
-        const uint32_t bytes = min(Tile::kTiles, p.scale_tiles - tile0) * 512;
-        mbar_arrive_expect_tx(&bars.full[s], Tile::kBytesP + bytes + (kFused ? 0 : Tile::kBytesQ + bytes * blocks_q));
-        tma_load_2d(smem_p + s * Tile::kBytesP, &map_p, kb * kRowBytes, p0, &bars.full[s]);
-        bulk_load(smem_sp + s * Tile::kBytesScaleP,
-                  p.sf_p + (static_cast<int64_t>(p0 / 128) * p.scale_tiles + tile0) * 512, bytes, &bars.full[s]);
-      };
-      const int ahead = min(p.stages, stages_here);
+    int blocks_q = 0;
+    for (int b = 0; b < Tile::kQBlocks; ++b) blocks_q += q0 + b * 128 < p.rows_q ? 1 : 0;
+    // The activations may come from the kernel in front of this one, the weight does not (a call's own
+    // quantiser is that kernel): the first stages of the weight are fetched before waiting.
+    auto load_p = [&](int i) {
+      const int kb = k_begin + i;
+      const int s = i % p.stages;
+      const int tile0 = kb * Tile::kTiles;
+      const uint32_t bytes = min(Tile::kTiles, p.scale_tiles - tile0) * 512;
+      mbar_arrive_expect_tx(&bars.full[s], Tile::kBytesP + bytes + (kFused ? 0 : Tile::kBytesQ + bytes * blocks_q));
+      tma_load_2d(smem_p + s * Tile::kBytesP, &map_p, kb * kRowBytes, p0, &bars.full[s]);
+      bulk_load(smem_sp + s * Tile::kBytesScaleP,
+                p.sf_p + (static_cast<int64_t>(p0 / 128) * p.scale_tiles + tile0) * 512, bytes, &bars.full[s]);
+    };
+    auto load_q = [&](int i) {
+      const int kb = k_begin + i;
+      const int s = i % p.stages;
+      const int tile0 = kb * Tile::kTiles;
+      const uint32_t bytes = min(Tile::kTiles, p.scale_tiles - tile0) * 512;
+      tma_load_2d(smem_q + s * Tile::kBytesQ, &map_q, kb * kRowBytes, q0, &bars.full[s]);
+      for (int b = 0; b < blocks_q; ++b) {
+        bulk_load(smem_sq + s * Tile::kBytesScaleQ + b * Tile::kTiles * 512,
+                  p.sf_q + (static_cast<int64_t>(q0 / 128 + b) * p.scale_tiles + tile0) * 512, bytes, &bars.full[s]);
+      }
+    };
+    const int ahead = min(p.stages, stages_here);
+    if (elect_one()) {
       for (int i = 0; i < ahead; ++i) load_p(i);
       if constexpr (!kFused) {
         pdl_wait_for_previous_kernel();
         for (int i = 0; i < ahead; ++i) load_q(i);
       }
-      for (int i = ahead; i < stages_here; ++i) {
-        mbar_wait_bounded(&bars.empty[i % p.stages], (i / p.stages - 1) & 1, abort_flag, p.status, kStatusStreamWait + 1);
-        if (*abort_flag) break;
+    }
+    __syncwarp();
+    for (int i = ahead; i < stages_here; ++i) {
+      if (!warp_wait(&bars.empty[i % p.stages], (i / p.stages - 1) & 1, abort_flag, p.status, kStatusStreamWait + 1)) break;
+      if (elect_one()) {
         load_p(i);
         if constexpr (!kFused) load_q(i);
       }
+      __syncwarp();
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      if constexpr (kFused) {
-        mbar_wait_bounded(&bars.x_ready, 0, abort_flag, p.status, kStatusStreamWait + 4);
-      }
-      for (int i = 0; i < stages_here; ++i) {
-        const int s = i % p.stages;
-        mbar_wait_bounded(&bars.full[s], (i / p.stages) & 1, abort_flag, p.status, kStatusStreamWait + 2);
-        if (*abort_flag) break;
-        tc_fence_after_sync();
-        const int sq = kFused ? i : s;
+    bool ok = true;
+    if constexpr (kFused) ok = warp_wait(&bars.x_ready, 0, abort_flag, p.status, kStatusStreamWait + 2);
+    for (int i = 0; ok && i < stages_here; ++i) {
+      const int s = i % p.stages;
+      ok = warp_wait(&bars.full[s], (i / p.stages) & 1, abort_flag, p.status, kStatusStreamWait + 3);
+      if (!ok) break;
+      tc_fence_after_sync();
+      const int sq = kFused ? i : s;
+      if (elect_one()) {
         issue_stage<kFormat, 1, kP, kQ>(tmem, tmem + kQ, smem_addr(smem_p + s * Tile::kBytesP),
                                         smem_addr(smem_q + sq * Tile::kBytesQ), smem_addr(smem_sp + s * Tile::kBytesScaleP),
                                         smem_addr(smem_sq + sq * Tile::kBytesScaleQ),
                                         p.cols_padded - (k_begin + i) * kStageCols, i == 0);
         mma_commit(&bars.empty[s]);
+        if (i == stages_here - 1) mma_commit(&bars.done);
       }
-      if (!*abort_flag) mma_commit(&bars.done);
+      __syncwarp();
     }
   } else {
     pdl_wait_for_previous_kernel();
@@ -235,7 +238,7 @@ __global__ void __launch_bounds__(StreamTile<kFormat, kQ, kFused>::kThreads, 1)
     }
     if (warp < 6) {
       // Every MMA of the CTA is complete, so the ring's memory holds the partial tile [kQ][128] now.
-      const bool ok = mbar_wait_bounded(&bars.done, 0, abort_flag, p.status, kStatusStreamWait + 3);
+      const bool ok = warp_wait(&bars.done, 0, abort_flag, p.status, kStatusStreamWait + 4);
       tc_fence_after_sync();
       if (ok) {
         const int quarter = warp & 3;

@@ -104,6 +104,53 @@ __device__ __forceinline__ void issue_stage(uint32_t d_tmem, uint32_t sf_tmem, u
   }
 }
 
+// Bounded wait that keeps polling: a warp parked with a time hint is not always woken early by an arrival
+// that comes from the tensor core or another CTA, and these kernels hand a stage on every 500 cycles.
+__device__ __forceinline__ bool mbar_spin_bounded(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                                                  int* status_word, int status_code) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long start = clock64();
+  while (true) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i) {
+      if (mbar_try_wait(bar, parity)) return true;
+    }
+    if (*abort_flag) return false;
+    if (clock64() - start > kWaitLimitCycles) {
+      *abort_flag = 1;
+      atomicCAS(status_word, 0, status_code);
+      return false;
+    }
+  }
+}
+
+// The same for all lanes of a warp, with one verdict: false when anybody has given up.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status_word,
+                                          int status_code) {
+  mbar_spin_bounded(bar, parity, abort_flag, status_word, status_code);
+  return __any_sync(0xffffffffu, *abort_flag) == 0;
+}
+
+// warp_wait for a barrier on which both CTAs of a pair arrive: what the other CTA did before its arrival is
+// ordered before what follows here.
+__device__ __forceinline__ bool warp_wait_pair(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                                               int* status_word, int status_code) {
+  const bool ok = warp_wait(bar, parity, abort_flag, status_word, status_code);
+  asm volatile("fence.acq_rel.cluster;" ::: "memory");
+  return ok;
+}
+
+// One lane of a converged warp.  The warps that issue copies and MMAs run their loops with all lanes and
+// choose one only around the instructions: addresses and descriptors are then the same for the warp as the
+// compiler sees it and stay in uniform registers.  In a branch on the lane number each tcgen05
+// instruction took 52-64 cycles to issue (a stage of four MMAs and six scale copies 629 cycles, NVFP4 with twelve
+// 932), with the elected lane the MMAs' own 512.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
 // ---- clusters --------------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
