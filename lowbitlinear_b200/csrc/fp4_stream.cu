@@ -37,15 +37,16 @@ struct StreamParams {
   int cols_padded;  // to 32
   int scale_tiles;  // along K
   int stages;
-  int split;        // CTAs of a cluster
+  int split;        // CTAs of a cluster, a power of two
+  int split_shift;  // its logarithm
   int x_vector;     // 16-byte loads of x allowed
+  int receive_offset;  // where partial sums arrive in shared memory; 0: over the ring
   int* status;
 };
 
 struct StreamBarriers {
   uint64_t full[kMaxStages];
   uint64_t empty[kMaxStages];
-  uint64_t x_ready;
   uint64_t done;
   uint32_t tmem_base;
   int abort_flag;
@@ -120,7 +121,7 @@ __device__ __forceinline__ void quantise_slice(const StreamParams& p, int k_begi
 }
 
 template <int kFormat, int kQ, bool kFused, typename T>
-__global__ void __launch_bounds__(StreamTile<kFormat, kQ, kFused>::kThreads, 1)
+__global__ void __launch_bounds__(StreamTile<kFormat, kQ, kFused>::kThreads, 2)
     fp4_stream_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
                       const StreamParams p) {
   using Tile = StreamTile<kFormat, kQ, kFused>;
@@ -132,11 +133,12 @@ __global__ void __launch_bounds__(StreamTile<kFormat, kQ, kFused>::kThreads, 1)
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const int lane = threadIdx.x & 31;
   const uint32_t rank = p.split > 1 ? cluster_rank() : 0;
-  const int p0 = (blockIdx.x / p.split) * kP;
+  const int p0 = (blockIdx.x >> p.split_shift) * kP;
   const int q0 = blockIdx.y * kQ;
+  const int used = min(kQ, p.rows_q - q0);  // activation rows of this tile
   const int k_stages = (p.cols_padded + kStageCols - 1) / kStageCols;
-  const int k_begin = static_cast<int>(static_cast<int64_t>(k_stages) * rank / p.split);
-  const int k_end = static_cast<int>(static_cast<int64_t>(k_stages) * (rank + 1) / p.split);
+  const int k_begin = static_cast<int>(static_cast<int64_t>(k_stages) * rank >> p.split_shift);
+  const int k_end = static_cast<int>(static_cast<int64_t>(k_stages) * (rank + 1) >> p.split_shift);
   const int stages_here = k_end - k_begin;
 
   // Code tiles first (swizzled tiles start on 1024 bytes).  kFused: Q holds the whole slice.
@@ -146,54 +148,43 @@ __global__ void __launch_bounds__(StreamTile<kFormat, kQ, kFused>::kThreads, 1)
   uint8_t* smem_sp = smem_q + q_slots * Tile::kBytesQ;
   uint8_t* smem_sq = smem_sp + p.stages * Tile::kBytesScaleP;
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < p.stages; ++s) {
-      mbar_init(&bars.full[s], 1);
-      mbar_init(&bars.empty[s], 1);
-    }
-    mbar_init(&bars.x_ready, Tile::kWorkers);
-    mbar_init(&bars.done, 1);
-    bars.abort_flag = 0;
-    mbar_init_fence();
-  }
-  if (warp == 1) {
-    tmem_alloc(&bars.tmem_base, Tile::kTmemColumns);
-    tmem_relinquish();
-  }
-  tc_fence_before_sync();
-  __syncthreads();
-  tc_fence_after_sync();
-  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&bars.tmem_base);
-  pdl_allow_next_kernel();
-
-  if (warp == 0) {
+  const int tile_step = Tile::kTiles;
+  auto load_p = [&](int i) {
+    const int kb = k_begin + i;
+    const int s = i % p.stages;
+    const uint32_t bytes = min(tile_step, p.scale_tiles - kb * tile_step) * 512;
     int blocks_q = 0;
-    for (int b = 0; b < Tile::kQBlocks; ++b) blocks_q += q0 + b * 128 < p.rows_q ? 1 : 0;
-    // The activations may come from the kernel in front of this one, the weight does not (a call's own
-    // quantiser is that kernel): the first stages of the weight are fetched before waiting.
-    auto load_p = [&](int i) {
-      const int kb = k_begin + i;
-      const int s = i % p.stages;
-      const int tile0 = kb * Tile::kTiles;
-      const uint32_t bytes = min(Tile::kTiles, p.scale_tiles - tile0) * 512;
-      mbar_arrive_expect_tx(&bars.full[s], Tile::kBytesP + bytes + (kFused ? 0 : Tile::kBytesQ + bytes * blocks_q));
-      tma_load_2d(smem_p + s * Tile::kBytesP, &map_p, kb * kRowBytes, p0, &bars.full[s]);
-      bulk_load(smem_sp + s * Tile::kBytesScaleP,
-                p.sf_p + (static_cast<int64_t>(p0 / 128) * p.scale_tiles + tile0) * 512, bytes, &bars.full[s]);
-    };
-    auto load_q = [&](int i) {
-      const int kb = k_begin + i;
-      const int s = i % p.stages;
-      const int tile0 = kb * Tile::kTiles;
-      const uint32_t bytes = min(Tile::kTiles, p.scale_tiles - tile0) * 512;
-      tma_load_2d(smem_q + s * Tile::kBytesQ, &map_q, kb * kRowBytes, q0, &bars.full[s]);
-      for (int b = 0; b < blocks_q; ++b) {
-        bulk_load(smem_sq + s * Tile::kBytesScaleQ + b * Tile::kTiles * 512,
-                  p.sf_q + (static_cast<int64_t>(q0 / 128 + b) * p.scale_tiles + tile0) * 512, bytes, &bars.full[s]);
-      }
-    };
-    const int ahead = min(p.stages, stages_here);
+    if (!kFused) {
+      for (int b = 0; b < Tile::kQBlocks; ++b) blocks_q += b * 128 < used ? 1 : 0;
+    }
+    mbar_arrive_expect_tx(&bars.full[s], Tile::kBytesP + bytes + (kFused ? 0 : Tile::kBytesQ + bytes * blocks_q));
+    tma_load_2d(smem_p + s * Tile::kBytesP, &map_p, kb * kRowBytes, p0, &bars.full[s]);
+    bulk_load(smem_sp + s * Tile::kBytesScaleP,
+              p.sf_p + (static_cast<int64_t>(p0 / 128) * p.scale_tiles + kb * tile_step) * 512, bytes, &bars.full[s]);
+  };
+  auto load_q = [&](int i) {
+    const int kb = k_begin + i;
+    const int s = i % p.stages;
+    const uint32_t bytes = min(tile_step, p.scale_tiles - kb * tile_step) * 512;
+    tma_load_2d(smem_q + s * Tile::kBytesQ, &map_q, kb * kRowBytes, q0, &bars.full[s]);
+    for (int b = 0; b < Tile::kQBlocks && b * 128 < used; ++b) {
+      bulk_load(smem_sq + s * Tile::kBytesScaleQ + b * tile_step * 512,
+                p.sf_q + (static_cast<int64_t>(q0 / 128 + b) * p.scale_tiles + kb * tile_step) * 512, bytes, &bars.full[s]);
+    }
+  };
+  const int ahead = min(p.stages, stages_here);
+
+  // The weight's first stages are on their way before anything else is set up.  The activations may come from
+  // the kernel in front of this one, the weight does not (a call's own quantiser is that kernel).
+  if (warp == 0) {
     if (elect_one()) {
+      for (int s = 0; s < p.stages; ++s) {
+        mbar_init(&bars.full[s], 1);
+        mbar_init(&bars.empty[s], 1);
+      }
+      mbar_init(&bars.done, 1);
+      bars.abort_flag = 0;
+      mbar_init_fence();
       for (int i = 0; i < ahead; ++i) load_p(i);
       if constexpr (!kFused) {
         pdl_wait_for_previous_kernel();
@@ -201,6 +192,26 @@ __global__ void __launch_bounds__(StreamTile<kFormat, kQ, kFused>::kThreads, 1)
       }
     }
     __syncwarp();
+  } else if (warp == 1) {
+    tmem_alloc(&bars.tmem_base, Tile::kTmemColumns);
+    tmem_relinquish();
+  } else {
+    pdl_wait_for_previous_kernel();
+    if constexpr (kFused) {
+      quantise_slice<kFormat, kQ, T>(p, k_begin, stages_here, smem_q, smem_sq, threadIdx.x - 64, Tile::kWorkers * 32);
+      fence_async_proxy();
+    }
+  }
+  // A partial sum may go to a neighbour once it has started (its receiving memory is its own) or, where that
+  // memory is the ring's, once its MMAs are complete.
+  if (p.split > 1 && p.receive_offset != 0) cluster_arrive();
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&bars.tmem_base);
+  pdl_allow_next_kernel();
+
+  if (warp == 0) {
     for (int i = ahead; i < stages_here; ++i) {
       if (!warp_wait(&bars.empty[i % p.stages], (i / p.stages - 1) & 1, abort_flag, p.status, kStatusStreamWait + 1)) break;
       if (elect_one()) {
@@ -210,12 +221,9 @@ __global__ void __launch_bounds__(StreamTile<kFormat, kQ, kFused>::kThreads, 1)
       __syncwarp();
     }
   } else if (warp == 1) {
-    bool ok = true;
-    if constexpr (kFused) ok = warp_wait(&bars.x_ready, 0, abort_flag, p.status, kStatusStreamWait + 2);
-    for (int i = 0; ok && i < stages_here; ++i) {
+    for (int i = 0; i < stages_here; ++i) {
       const int s = i % p.stages;
-      ok = warp_wait(&bars.full[s], (i / p.stages) & 1, abort_flag, p.status, kStatusStreamWait + 3);
-      if (!ok) break;
+      if (!warp_wait(&bars.full[s], (i / p.stages) & 1, abort_flag, p.status, kStatusStreamWait + 2)) break;
       tc_fence_after_sync();
       const int sq = kFused ? i : s;
       if (elect_one()) {
@@ -228,46 +236,54 @@ __global__ void __launch_bounds__(StreamTile<kFormat, kQ, kFused>::kThreads, 1)
       }
       __syncwarp();
     }
-  } else {
-    pdl_wait_for_previous_kernel();
-    if constexpr (kFused) {
-      quantise_slice<kFormat, kQ, T>(p, k_begin, stages_here, smem_q, smem_sq, threadIdx.x - 64, Tile::kWorkers * 32);
-      fence_async_proxy();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.x_ready);
-    }
-    if (warp < 6) {
-      // Every MMA of the CTA is complete, so the ring's memory holds the partial tile [kQ][128] now.
-      const bool ok = warp_wait(&bars.done, 0, abort_flag, p.status, kStatusStreamWait + 4);
-      tc_fence_after_sync();
-      if (ok) {
-        const int quarter = warp & 3;
-        const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-        float* partial = reinterpret_cast<float*>(smem) + quarter * 32 + lane;
-        const int used = min(kQ, p.rows_q - q0);
-        for (int c0 = 0; c0 < used; c0 += 32) {
-          uint32_t v[32];
-          tmem_load_32cols(taddr + c0, v);
-          tmem_load_wait();
-#pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            if (c0 + c < kQ) partial[(c0 + c) * kP] = __uint_as_float(v[c]);
-          }
-        }
-      }
-    }
   }
-
+  // When this barrier has passed every MMA of the CTA is complete and every copy has been read.
+  warp_wait(&bars.done, 0, abort_flag, p.status, kStatusStreamWait + 3);
+  tc_fence_after_sync();
   if (*abort_flag) {
-    // Give copies that are still in flight time to land before the shared memory is released.
+    // Give copies that are still in flight time to land before the shared memory is used otherwise.
     const long long start = clock64();
     while (clock64() - start < 200000) {
     }
   }
-  tc_fence_before_sync();
-  __syncwarp();
+  __syncthreads();
   if (p.split > 1) {
-    cluster_sync_all();
+    if (p.receive_offset == 0) cluster_arrive();
+    cluster_wait();
+  }
+
+  // Row q of the tile is summed by CTA q % split, which receives [slice][q / split][128] FP32.
+  const int slots = kQ >> p.split_shift;
+  uint8_t* received = smem + p.receive_offset;
+  if (warp >= 2 && warp < 6) {
+    const int quarter = warp & 3;
+    const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    const uint32_t mine = smem_addr(received) + (rank * slots * kP + quarter * 32 + lane) * 4;
+    for (int c0 = 0; c0 < used; c0 += 32) {
+      uint32_t v[32];
+      tmem_load_32cols(taddr + c0, v);
+      tmem_load_wait();
+      if (p.split == 1) {
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          if (c0 + c >= used) break;
+          asm volatile("st.shared::cta.b32 [%0], %1;" ::"r"(mine + (c0 + c) * kP * 4), "r"(v[c]) : "memory");
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          const int q = c0 + c;
+          if (q >= used) break;
+          const uint32_t to = map_to_cta(mine + (q >> p.split_shift) * kP * 4, q & (p.split - 1));
+          asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(to), "r"(v[c]) : "memory");
+        }
+      }
+    }
+  }
+  tc_fence_before_sync();
+  if (p.split > 1) {
+    cluster_arrive();
+    cluster_wait();
   } else {
     __syncthreads();
   }
@@ -276,27 +292,21 @@ __global__ void __launch_bounds__(StreamTile<kFormat, kQ, kFused>::kThreads, 1)
     tmem_dealloc(tmem, Tile::kTmemColumns);
   }
 
-  // Two neighbouring rows of the weight and one activation row per thread and step; the cluster's CTAs share
-  // the tile, and each adds the slices in their order.
+  // Two neighbouring rows of the weight and one activation row per thread and step; slices in their order.
   const float alpha = product_factor(p.factor_p, p.factor_q);
-  const int used = min(kQ, p.rows_q - q0);
-  const uint32_t partial_addr = smem_addr(smem);
   T* out = static_cast<T*>(p.out);
   const bool paired = (p.out_pitch & 1) == 0 && (reinterpret_cast<uintptr_t>(out) & 3) == 0;
-  for (int item = rank * Tile::kThreads + threadIdx.x; item < used * (kP / 2); item += p.split * Tile::kThreads) {
-    const int q = item / (kP / 2);
+  const int my_rows = used > static_cast<int>(rank) ? (used - static_cast<int>(rank) + p.split - 1) >> p.split_shift : 0;
+  for (int item = threadIdx.x; item < my_rows * (kP / 2); item += Tile::kThreads) {
+    const int slot = item / (kP / 2);
     const int row = (item % (kP / 2)) * 2;
-    const uint32_t offset = partial_addr + (q * kP + row) * 4;
+    const int q = (slot << p.split_shift) + rank;
+    const float2* part = reinterpret_cast<const float2*>(received) + (slot * kP + row) / 2;
     float a = 0.0f, b = 0.0f;
-    if (p.split > 1) {
-      for (int r = 0; r < p.split; ++r) {
-        float2 v;
-        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(map_to_cta(offset, r)) : "memory");
-        a += v.x, b += v.y;
-      }
-    } else {
-      const float2 v = *reinterpret_cast<const float2*>(smem + (q * kP + row) * 4);
-      a = v.x, b = v.y;
+#pragma unroll 4
+    for (int r = 0; r < p.split; ++r) {
+      const float2 v = part[r * slots * (kP / 2)];
+      a += v.x, b += v.y;
     }
     if (p0 + row >= p.rows_p) continue;
     T* dst = out + (q0 + q) * p.out_pitch + p0 + row;
@@ -308,14 +318,28 @@ __global__ void __launch_bounds__(StreamTile<kFormat, kQ, kFused>::kThreads, 1)
       if (p0 + row + 1 < p.rows_p) *(reinterpret_cast<unsigned short*>(dst) + 1) = static_cast<unsigned short>(y >> 16);
     }
   }
-  // Nobody leaves while a neighbour may still read its partial tile.
-  __syncwarp();
-  if (p.split > 1) cluster_sync_all();
 }
 
-constexpr int kSmemLimit = 227 * 1024;
+constexpr int kSmemLimit = 226 * 1024;     // dynamic shared memory of a CTA
+constexpr int kSmemPerSm = 228 * 1024;
 constexpr int kFusedRows = 16;
-constexpr int kFusedSliceBytes = 64 * 1024;
+constexpr int kFusedUnits = 512;  // of sixteen columns: what the quantising warps of a CTA round in two steps
+constexpr int kRingStages = 6;
+
+// Slices of K, each on a CTA of its own: doubled until most SMs have one, and beyond that while a slice keeps four
+// stages (a second CTA on an SM hides the first one's start, but the sums cost more to join).  Measured, us, 1 / 2 /
+// 4 / 8 slices: 32 row blocks of 16 stages 8.9 / 7.1 / 5.5 / 5.8, of 48 stages 23 / 14 / 9.3 / 8.5; 48 blocks of 16
+// stages 12.6 / 9.7 / 8.2 / 10.2; 192 blocks of 16 stages 14.5 / 14.2 / 16.7 / 20.7.
+int choose_split(int64_t tiles, int k_stages, int sm_count) {
+  int split = 1;
+  while (split < kMaxSplit && k_stages >= 2 * split &&
+         (5 * tiles * split < 4 * sm_count || (tiles * split < sm_count && k_stages >= 8 * split))) {
+    split *= 2;
+  }
+  return split;
+}
+
+int stages_of(int64_t K) { return static_cast<int>((fp4::padded_cols(K) + kStageCols - 1) / kStageCols); }
 
 template <int kFormat, int kQ, bool kFused, typename T>
 cudaError_t launch(const Fp4Operand& w, const Fp4Operand& x, const void* raw, int64_t raw_stride, void* out, int64_t K,
@@ -331,14 +355,8 @@ cudaError_t launch(const Fp4Operand& w, const Fp4Operand& x, const void* raw, in
   }
   const int64_t blocks_p = (w.rows + kP - 1) / kP;
   const int64_t blocks_q = (x.rows + kQ - 1) / kQ;
-  const int k_stages = static_cast<int>((fp4::padded_cols(K) + kStageCols - 1) / kStageCols);
-  // Slices until the SMs are busy, two stages at least in each.
-  int split = 1;
-  while (split < kMaxSplit && blocks_p * blocks_q * split * 2 <= 2 * sm_count && k_stages >= split * 4) split *= 2;
-  if constexpr (kFused) {
-    // The slice of the activations shares the memory with the ring.
-    while (split < kMaxSplit && (k_stages + split - 1) / split * (Tile::kBytesQ + Tile::kBytesScaleQ) > kFusedSliceBytes) split *= 2;
-  }
+  const int k_stages = stages_of(K);
+  const int split = choose_split(blocks_p * blocks_q, k_stages, sm_count);
   const int slice = (k_stages + split - 1) / split;
 
   StreamParams params;
@@ -356,15 +374,25 @@ cudaError_t launch(const Fp4Operand& w, const Fp4Operand& x, const void* raw, in
   params.cols_padded = static_cast<int>(fp4::padded_cols(K));
   params.scale_tiles = static_cast<int>(fp4::scale_tiles(K, kFormat));
   params.split = split;
+  params.split_shift = 0;
+  while ((1 << params.split_shift) < split) ++params.split_shift;
   params.x_vector = (raw_stride * 2) % 16 == 0 && reinterpret_cast<uintptr_t>(raw) % 16 == 0;
   params.status = status;
-  const int fixed = 1024 + (kFused ? slice * (Tile::kBytesQ + Tile::kBytesScaleQ) : 0);
-  int stages = slice < 6 ? slice : 6;
-  while (stages > 1 && fixed + stages * Tile::kStageBytes > kSmemLimit - 1024) --stages;
+  // Received partial sums have memory of their own while they are small, and lie over the ring otherwise.
+  const bool own_memory = split > 1 && kQ <= 32;
+  const int fixed = 1024 + (kFused ? slice * (Tile::kBytesQ + Tile::kBytesScaleQ) : 0) + (own_memory ? Tile::kPartialBytes : 0);
+  // All CTAs on the SMs at once where that leaves two stages: a CTA that has to wait for another one's end starts
+  // its pipeline cold.  At least two on an SM in any case, for the next kernel of the stream.
+  const int64_t ctas = blocks_p * blocks_q * split;
+  const int64_t per_sm = ctas <= 2 * sm_count ? 2 : ctas <= 3 * sm_count ? 3 : 4;
+  const int budget = static_cast<int>(kSmemPerSm / per_sm) - 1024;  // the driver takes 1 KB of each CTA's share
+  int stages = slice < kRingStages ? slice : kRingStages;
+  while (stages > 2 && fixed + stages * Tile::kStageBytes > budget) --stages;
   params.stages = stages;
   int smem = fixed + stages * Tile::kStageBytes;
+  params.receive_offset = own_memory ? smem - 1024 - Tile::kPartialBytes : 0;
   if (smem < Tile::kPartialBytes + 1024) smem = Tile::kPartialBytes + 1024;
-  if (smem > kSmemLimit - 1024) return cudaErrorInvalidValue;
+  if (smem > kSmemLimit) return cudaErrorInvalidValue;
 
   auto kernel = fp4_stream_kernel<kFormat, kQ, kFused, T>;
   static bool configured[64] = {};
@@ -372,7 +400,7 @@ cudaError_t launch(const Fp4Operand& w, const Fp4Operand& x, const void* raw, in
   cudaError_t err = cudaGetDevice(&device);
   if (err != cudaSuccess) return err;
   if (device < 0 || device >= 64 || !configured[device]) {
-    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit - 1024);
+    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
     if (err != cudaSuccess) return err;
     if (device >= 0 && device < 64) configured[device] = true;
   }
@@ -406,6 +434,7 @@ cudaError_t launch(const Fp4Operand& w, const Fp4Operand& x, const void* raw, in
 template <int kFormat, typename T>
 static cudaError_t stream_product(const Fp4Operand& a, const Fp4Operand& b, void* out, int64_t K, int sm_count,
                                   int* status, bool pdl, cudaStream_t stream) {
+  if (a.rows <= 16) return launch<kFormat, 16, false, T>(b, a, nullptr, 0, out, K, sm_count, status, pdl, stream);
   if (a.rows <= 32) return launch<kFormat, 32, false, T>(b, a, nullptr, 0, out, K, sm_count, status, pdl, stream);
   if (a.rows <= 64) return launch<kFormat, 64, false, T>(b, a, nullptr, 0, out, K, sm_count, status, pdl, stream);
   return launch<kFormat, 128, false, T>(b, a, nullptr, 0, out, K, sm_count, status, pdl, stream);
@@ -421,10 +450,12 @@ cudaError_t launch_fp4_stream(const Fp4Operand& a, const Fp4Operand& b, int form
                                : stream_product<fp4::kMx, __half>(a, b, out, K, sm_count, status_word, pdl, stream);
 }
 
-bool fp4_fused_supports(int64_t M, int64_t K, int format) {
-  const int64_t k_stages = (fp4::padded_cols(K) + kStageCols - 1) / kStageCols;
-  const int64_t stage_bytes = kFusedRows * kRowBytes + (format == fp4::kNv ? 4 : 2) * 512;
-  return M <= kFusedRows && (k_stages + kMaxSplit - 1) / kMaxSplit * stage_bytes <= kFusedSliceBytes;
+// Every CTA rounds its slice of the activations itself: worth a launch while that is a step or two.
+bool fp4_fused_supports(int64_t M, int64_t N, int64_t K, int sm_count) {
+  if (M > kFusedRows) return false;
+  const int64_t k_stages = stages_of(K);
+  const int split = choose_split((N + kP - 1) / kP, static_cast<int>(k_stages), sm_count);
+  return M * 16 * ((k_stages + split - 1) / split) <= kFusedUnits;
 }
 
 cudaError_t launch_fp4_fused_linear(const void* x, int x_type, int64_t x_stride, int64_t M, const float* x_factor,
