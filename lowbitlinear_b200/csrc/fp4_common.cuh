@@ -176,21 +176,53 @@ __device__ __forceinline__ float step_of(uint32_t byte, float g) {
 }
 
 // ---- sixteen neighbouring activations or weights as they lie in memory -------------------------
+// How the rows of a matrix may be read or written, by the alignment of its base and pitch.
+constexpr int kRows32 = 2;  // 32-byte accesses
+constexpr int kRows16 = 1;  // 16-byte accesses
+constexpr int kRowsAny = 0;
+inline int row_access(const void* base, int64_t pitch_bytes) {
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(base) | static_cast<uintptr_t>(pitch_bytes);
+  return bits % 32 == 0 ? kRows32 : bits % 16 == 0 ? kRows16 : kRowsAny;
+}
+
+// 32 bytes in one access (the address a multiple of 32).  With two 16-byte accesses per lane each
+// touches half of every 32-byte sector it reaches.
+__device__ __forceinline__ void load_32_bytes(const void* p, uint32_t (&w)[8]) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+      : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+      : "l"(p));
+}
+__device__ __forceinline__ void store_32_bytes(void* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
 template <typename T>
 struct Sixteen;
 template <>
 struct Sixteen<float> {
   float v[16];
-  __device__ __forceinline__ void load_vector(const float* p) {
+  __device__ __forceinline__ void load_vector(const float* p, int access) {
+    if (access == kRows32) {
+      uint32_t w[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float4 q = __ldg(reinterpret_cast<const float4*>(p) + i);
-      v[4 * i] = q.x, v[4 * i + 1] = q.y, v[4 * i + 2] = q.z, v[4 * i + 3] = q.w;
+      for (int h = 0; h < 2; ++h) {
+        load_32_bytes(p + 8 * h, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[8 * h + i] = __uint_as_float(w[i]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float4 q = reinterpret_cast<const float4*>(p)[i];
+        v[4 * i] = q.x, v[4 * i + 1] = q.y, v[4 * i + 2] = q.z, v[4 * i + 3] = q.w;
+      }
     }
   }
   __device__ __forceinline__ void load_masked(const float* p, int valid) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = i < valid ? __ldg(p + i) : 0.0f;
+    for (int i = 0; i < 16; ++i) v[i] = i < valid ? p[i] : 0.0f;
   }
   // Bits of the largest magnitude as FP32; integer order, so that NaN beats infinity beats all.
   __device__ __forceinline__ uint32_t amax_bits() const {
@@ -219,17 +251,21 @@ __device__ __forceinline__ float2 pair_to_float<__nv_bfloat16>(uint32_t bits) {
 template <typename T>
 struct SixteenHalves {
   uint32_t w[8];
-  __device__ __forceinline__ void load_vector(const T* p) {
-    const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
-    const uint4 b = __ldg(reinterpret_cast<const uint4*>(p) + 1);
-    w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+  __device__ __forceinline__ void load_vector(const T* p, int access) {
+    if (access == kRows32) {
+      load_32_bytes(p, w);
+    } else {
+      const uint4 a = reinterpret_cast<const uint4*>(p)[0];
+      const uint4 b = reinterpret_cast<const uint4*>(p)[1];
+      w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+    }
   }
   __device__ __forceinline__ void load_masked(const T* p, int valid) {
     const unsigned short* raw = reinterpret_cast<const unsigned short*>(p);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const uint32_t lo = 2 * i < valid ? __ldg(raw + 2 * i) : 0u;
-      const uint32_t hi = 2 * i + 1 < valid ? __ldg(raw + 2 * i + 1) : 0u;
+      const uint32_t lo = 2 * i < valid ? raw[2 * i] : 0u;
+      const uint32_t hi = 2 * i + 1 < valid ? raw[2 * i + 1] : 0u;
       w[i] = lo | (hi << 16);
     }
   }

@@ -15,6 +15,12 @@
 // Tensor memory holds two accumulators of 256 columns that overlap, [0, 256) and [208, 464), beside the 48 columns
 // of scales.  The epilogue reads the shared columns of a tile first and gives them back at once; the next
 // tile's MMAs start then and run beside the rest of the epilogue.
+//
+// kSplit: fewer tiles than half the pairs of SMs.  One SM takes in 45 bytes per cycle, so a tile on its own needs 7 us
+// for 4096 columns of K; two pairs of a cluster share it then, each with half of K, push the FP32 sums of the columns
+// they do not own to the pair that does (distributed shared memory, over the ring that has been read), and both
+// pairs add and store their columns, always in the same order.  (256 x 6144 x 4096: 11.5 us, 13.4 without.  Four
+// pairs, clusters of eight CTAs with 200 KB each, took 20 us: too few of them fit on the chip at once.)
 #include "fp4_tc.cuh"
 
 namespace lbl {
@@ -80,13 +86,13 @@ __device__ __forceinline__ void tmem_relinquish_pair() {
 __device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t cols) {
   asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
 }
-// Arrives on the barrier at this shared-memory offset in both CTAs of the pair once every MMA
-// issued so far has finished.
-__device__ __forceinline__ void mma_commit_pair(uint64_t* bar) {
+// Arrives on the barrier at this shared-memory offset in both CTAs of the pair (cluster ranks `leader` and
+// leader + 1) once every MMA issued so far has finished.
+__device__ __forceinline__ void mma_commit_pair(uint64_t* bar, uint32_t leader) {
   asm volatile(
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
           smem_addr(bar)),
-      "h"(static_cast<uint16_t>(3))
+      "h"(static_cast<uint16_t>(3u << leader))
       : "memory");
 }
 // Tiled load into this CTA's shared memory that completes on a barrier of the pair's first CTA.
@@ -112,7 +118,49 @@ __device__ __forceinline__ void tile_of(const PairParams& p, int t, int* tile_a,
   *tile_b = rest / rows;
 }
 
-template <int kFormat, typename T>
+// One warp's 32 rows x 64 columns of sums, a row per lane, to out through the warp's staging memory, so that rows leave
+// as whole 128-byte runs.
+template <typename T>
+__device__ __forceinline__ void store_chunk(const PairParams& p, const uint32_t (&v)[2][32], float alpha,
+                                            uint8_t* staging, int row0, int col0, int lane) {
+  // Row `lane`: eight pieces of 16 bytes, swizzled over the banks.
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t* f = &v[i >> 2][(i & 3) * 8];
+    uint4 q;
+    q.x = two_rounded<T>(__uint_as_float(f[0]) * alpha, __uint_as_float(f[1]) * alpha);
+    q.y = two_rounded<T>(__uint_as_float(f[2]) * alpha, __uint_as_float(f[3]) * alpha);
+    q.z = two_rounded<T>(__uint_as_float(f[4]) * alpha, __uint_as_float(f[5]) * alpha);
+    q.w = two_rounded<T>(__uint_as_float(f[6]) * alpha, __uint_as_float(f[7]) * alpha);
+    *reinterpret_cast<uint4*>(staging + lane * 128 + ((i ^ (lane & 7)) << 4)) = q;
+  }
+  __syncwarp();
+  T* out = static_cast<T*>(p.out);
+  const int piece = lane & 7;
+  const int col = col0 + piece * 8;
+#pragma unroll
+  for (int r = lane >> 3; r < 32; r += 4) {
+    const uint4 q = *reinterpret_cast<const uint4*>(staging + r * 128 + ((piece ^ (r & 7)) << 4));
+    const int row = row0 + r;
+    if (row < p.rows_a && col < p.rows_b) {
+      T* dst = out + row * p.out_pitch + col;
+      if (p.vector_ok && col + 8 <= p.rows_b) {
+        *reinterpret_cast<uint4*>(dst) = q;
+      } else {
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (col + e < p.rows_b) {
+            reinterpret_cast<unsigned short*>(dst)[e] = static_cast<unsigned short>(w[e >> 1] >> (16 * (e & 1)));
+          }
+        }
+      }
+    }
+  }
+  __syncwarp();
+}
+
+template <int kFormat, bool kSplit, typename T>
 __global__ void __launch_bounds__(kThreads, 1)
     fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                     const __grid_constant__ CUtensorMap map_sa, const __grid_constant__ CUtensorMap map_sb,
@@ -130,11 +178,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* abort_flag = &bars.abort_flag;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const int lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_rank();  // 0: issues the MMAs
-  const int first_tile = blockIdx.x >> 1;
-  const int tile_step = gridDim.x >> 1;
+  const uint32_t in_cluster = cluster_rank();
+  const uint32_t rank = in_cluster & 1;        // in the pair; 0 issues the MMAs
+  const uint32_t leader = in_cluster & ~1u;    // cluster rank of the pair's first CTA
+  const int slice = kSplit ? static_cast<int>(in_cluster >> 1) : 0;
+  const int first_tile = kSplit ? blockIdx.x >> 2 : blockIdx.x >> 1;
   const int tiles = p.tiles_a * p.tiles_b;
+  const int tile_step = kSplit ? tiles : gridDim.x >> 1;  // kSplit: one tile per cluster
   const int k_stages = (p.cols_padded + kStageCols - 1) / kStageCols;
+  const int kb_begin = kSplit ? k_stages * slice / 2 : 0;
+  const int kb_end = kSplit ? k_stages * (slice + 1) / 2 : k_stages;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < Tile::kStages; ++s) {
@@ -145,6 +198,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&bars.acc_free, 2 * kEpilogueWarps);
     bars.abort_flag = 0;
     mbar_init_fence();
+  }
+  if (warp == 0 && elect_one()) {
+    prefetch_map(&map_a);
+    prefetch_map(&map_b);
+    prefetch_map(&map_sa);
+    prefetch_map(&map_sb);
   }
   if (warp == 1) {
     tmem_alloc_pair(&bars.tmem_base, kTmemColumns);
@@ -160,7 +219,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == 0) {
     pdl_wait_for_previous_kernel();
-    const uint32_t full = map_to_cta(smem_addr(&bars.full[0]), 0);
+    const uint32_t full = map_to_cta(smem_addr(&bars.full[0]), leader);
     int i = 0;  // stages since the start
     for (int t = first_tile; t < tiles; t += tile_step) {
       int tile_a, tile_b;
@@ -169,7 +228,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int row_a = tile_a * kRowsPair + static_cast<int>(rank) * kRowsCta;
       const int row_b = tile_b * kRowsPair + static_cast<int>(rank) * kRowsCta;
       bool ok = true;
-      for (int kb = 0; kb < k_stages; ++kb, ++i) {
+      for (int kb = kb_begin; kb < kb_end; ++kb, ++i) {
         const int s = i % Tile::kStages;
         const int round = i / Tile::kStages;
         ok = round == 0 || warp_wait(&bars.empty[s], (round - 1) & 1, abort_flag, p.status, kStatusPairWait + 1);
@@ -196,7 +255,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         tc_fence_after_sync();
         const uint32_t acc = tmem + (n & 1) * kSecondAccumulator;
-        for (int kb = 0; kb < k_stages; ++kb, ++i) {
+        for (int kb = kb_begin; kb < kb_end; ++kb, ++i) {
           const int s = i % Tile::kStages;
           ok = warp_wait(&bars.full[s], (i / Tile::kStages) & 1, abort_flag, p.status, kStatusPairWait + 3);
           if (!ok) break;
@@ -205,22 +264,21 @@ __global__ void __launch_bounds__(kThreads, 1)
             issue_stage<kFormat, 2, kRowsPair, kRowsPair>(
                 acc, tmem + kScaleColumn, smem_addr(smem_a + s * Tile::kBytesCodes),
                 smem_addr(smem_b + s * Tile::kBytesCodes), smem_addr(smem_sa + s * Tile::kBytesScaleA),
-                smem_addr(smem_sb + s * Tile::kBytesScaleB), p.cols_padded - kb * kStageCols, kb == 0);
-            mma_commit_pair(&bars.empty[s]);
-            if (kb == k_stages - 1) mma_commit_pair(&bars.acc_full);
+                smem_addr(smem_sb + s * Tile::kBytesScaleB), p.cols_padded - kb * kStageCols, kb == kb_begin);
+            mma_commit_pair(&bars.empty[s], leader);
+            if (kb == kb_end - 1) mma_commit_pair(&bars.acc_full, leader);
           }
           __syncwarp();
         }
         if (!ok) break;
       }
     }
-  } else {
+  } else if constexpr (!kSplit) {
     pdl_wait_for_previous_kernel();
     const float alpha = product_factor(p.factor_a, p.factor_b);
-    const uint32_t acc_free = map_to_cta(smem_addr(&bars.acc_free), 0);
+    const uint32_t acc_free = map_to_cta(smem_addr(&bars.acc_free), leader);
     const int quarter = warp & 3;
     uint8_t* mine = staging + (warp - 2) * kStagingBytes;
-    T* out = static_cast<T*>(p.out);
     int n = 0;
     for (int t = first_tile; t < tiles; t += tile_step, ++n) {
       int tile_a, tile_b;
@@ -243,40 +301,61 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
           if (lane == 0) arrive_remote(acc_free);
         }
-        // Row `lane` of the chunk: eight pieces of 16 bytes, swizzled over the banks.
+        store_chunk<T>(p, v, alpha, mine, row0, col0 + first_col, lane);
+      }
+    }
+  }
+
+  if constexpr (kSplit) {
+    constexpr int kOwnChunks = kRowsPair / kChunk / 2;  // a pair stores half of the columns
+    const int quarter = warp & 3;
+    const uint32_t acc = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    bool ok = false;
+    if (warp >= 2) {
+      pdl_wait_for_previous_kernel();
+      ok = warp_wait(&bars.acc_full, 0, abort_flag, p.status, kStatusPairWait + 4);
+      tc_fence_after_sync();
+    }
+    // Every CTA of the cluster has read its ring to the end: the other pair's sums may land there,
+    // [own chunks][64 columns][128 rows] FP32.
+    __syncwarp();
+    cluster_sync_all();
+    const uint32_t place = smem_addr(smem) + static_cast<uint32_t>(quarter * 32 + lane) * 4;
+    if (ok) {
+#pragma unroll 1
+      for (int c = 0; c < kOwnChunks; ++c) {
+        const int column = ((1 - slice) * kOwnChunks + c) * kChunk;
+        const uint32_t to = map_to_cta(place + static_cast<uint32_t>(c) * (kChunk * kRowsCta * 4), in_cluster ^ 2u);
+        uint32_t v[2][32];
+        tmem_load_32cols(acc + column, v[0]);
+        tmem_load_32cols(acc + column + 32, v[1]);
+        tmem_load_wait();
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint32_t* f = &v[i >> 2][(i & 3) * 8];
-          uint4 q;
-          q.x = two_rounded<T>(__uint_as_float(f[0]) * alpha, __uint_as_float(f[1]) * alpha);
-          q.y = two_rounded<T>(__uint_as_float(f[2]) * alpha, __uint_as_float(f[3]) * alpha);
-          q.z = two_rounded<T>(__uint_as_float(f[4]) * alpha, __uint_as_float(f[5]) * alpha);
-          q.w = two_rounded<T>(__uint_as_float(f[6]) * alpha, __uint_as_float(f[7]) * alpha);
-          *reinterpret_cast<uint4*>(mine + lane * 128 + ((i ^ (lane & 7)) << 4)) = q;
+        for (int j = 0; j < kChunk; ++j) {
+          asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(to + j * kRowsCta * 4), "r"(v[j >> 5][j & 31]) : "memory");
         }
-        __syncwarp();
-        const int piece = lane & 7;
-        const int col = col0 + first_col + piece * 8;
+      }
+    }
+    __syncwarp();
+    cluster_sync_all();
+    if (ok) {
+      const float alpha = product_factor(p.factor_a, p.factor_b);
+      int tile_a, tile_b;
+      tile_of(p, first_tile, &tile_a, &tile_b);
+      const int row0 = tile_a * kRowsPair + static_cast<int>(rank) * kRowsCta + quarter * 32;
+#pragma unroll 1
+      for (int c = 0; c < kOwnChunks; ++c) {
+        const int column = (slice * kOwnChunks + c) * kChunk;
+        uint32_t v[2][32];
+        tmem_load_32cols(acc + column, v[0]);
+        tmem_load_32cols(acc + column + 32, v[1]);
+        tmem_load_wait();
+        const float* part = reinterpret_cast<const float*>(smem) + c * (kChunk * kRowsCta) + quarter * 32 + lane;
 #pragma unroll
-        for (int r = lane >> 3; r < 32; r += 4) {
-          const uint4 q = *reinterpret_cast<const uint4*>(mine + r * 128 + ((piece ^ (r & 7)) << 4));
-          const int row = row0 + r;
-          if (row < p.rows_a && col < p.rows_b) {
-            T* dst = out + row * p.out_pitch + col;
-            if (p.vector_ok && col + 8 <= p.rows_b) {
-              *reinterpret_cast<uint4*>(dst) = q;
-            } else {
-              const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                if (col + e < p.rows_b) {
-                  reinterpret_cast<unsigned short*>(dst)[e] = static_cast<unsigned short>(w[e >> 1] >> (16 * (e & 1)));
-                }
-              }
-            }
-          }
+        for (int j = 0; j < kChunk; ++j) {
+          v[j >> 5][j & 31] = __float_as_uint(__uint_as_float(v[j >> 5][j & 31]) + part[j * kRowsCta]);
         }
-        __syncwarp();
+        store_chunk<T>(p, v, alpha, staging + (warp - 2) * kStagingBytes, row0, tile_b * kRowsPair + column, lane);
       }
     }
   }
@@ -308,7 +387,7 @@ bool encode_scales(CUtensorMap* map, const uint8_t* scales, int64_t rows, int64_
                            CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
-template <int kFormat, typename T>
+template <int kFormat, bool kSplit, typename T>
 cudaError_t launch(const Fp4Operand& a, const Fp4Operand& b, void* out, int64_t K, int sm_count, int* status, bool pdl,
                    cudaStream_t stream) {
   using Tile = PairTile<kFormat>;
@@ -334,7 +413,7 @@ cudaError_t launch(const Fp4Operand& a, const Fp4Operand& b, void* out, int64_t 
   params.vector_ok = b.rows % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
   params.status = status;
 
-  auto kernel = fp4_pair_kernel<kFormat, T>;
+  auto kernel = fp4_pair_kernel<kFormat, kSplit, T>;
   static bool configured[64] = {};
   int device = 0;
   cudaError_t err = cudaGetDevice(&device);
@@ -345,7 +424,8 @@ cudaError_t launch(const Fp4Operand& a, const Fp4Operand& b, void* out, int64_t 
     if (device >= 0 && device < 64) configured[device] = true;
   }
   const int64_t slots = sm_count >= 2 ? sm_count / 2 : 1;
-  const int64_t pairs = tiles_a * tiles_b < slots ? tiles_a * tiles_b : slots;
+  int64_t pairs = tiles_a * tiles_b < slots ? tiles_a * tiles_b : slots;
+  if (kSplit) pairs = 2 * tiles_a * tiles_b;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs));
   cfg.blockDim = dim3(kThreads);
@@ -353,7 +433,7 @@ cudaError_t launch(const Fp4Operand& a, const Fp4Operand& b, void* out, int64_t 
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.x = kSplit ? 4 : 2;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -363,16 +443,25 @@ cudaError_t launch(const Fp4Operand& a, const Fp4Operand& b, void* out, int64_t 
   return cudaLaunchKernelEx(&cfg, kernel, map_a, map_b, map_sa, map_sb, params);
 }
 
+template <int kFormat, typename T>
+cudaError_t pair_product(const Fp4Operand& a, const Fp4Operand& b, void* out, int64_t K, int sm_count, int* status,
+                         bool pdl, cudaStream_t stream) {
+  const int64_t tiles = ((a.rows + kRowsPair - 1) / kRowsPair) * ((b.rows + kRowsPair - 1) / kRowsPair);
+  const bool split = 2 * tiles <= sm_count / 2 && fp4::padded_cols(K) > 3 * kStageCols;
+  return split ? launch<kFormat, true, T>(a, b, out, K, sm_count, status, pdl, stream)
+               : launch<kFormat, false, T>(a, b, out, K, sm_count, status, pdl, stream);
+}
+
 }  // namespace
 
 cudaError_t launch_fp4_pair(const Fp4Operand& a, const Fp4Operand& b, int format, void* out, int out_type, int64_t K,
                             int sm_count, int* status_word, bool pdl, cudaStream_t stream) {
   if (format == fp4::kNv) {
-    return out_type == kTypeBf16 ? launch<fp4::kNv, __nv_bfloat16>(a, b, out, K, sm_count, status_word, pdl, stream)
-                                 : launch<fp4::kNv, __half>(a, b, out, K, sm_count, status_word, pdl, stream);
+    return out_type == kTypeBf16 ? pair_product<fp4::kNv, __nv_bfloat16>(a, b, out, K, sm_count, status_word, pdl, stream)
+                                 : pair_product<fp4::kNv, __half>(a, b, out, K, sm_count, status_word, pdl, stream);
   }
-  return out_type == kTypeBf16 ? launch<fp4::kMx, __nv_bfloat16>(a, b, out, K, sm_count, status_word, pdl, stream)
-                               : launch<fp4::kMx, __half>(a, b, out, K, sm_count, status_word, pdl, stream);
+  return out_type == kTypeBf16 ? pair_product<fp4::kMx, __nv_bfloat16>(a, b, out, K, sm_count, status_word, pdl, stream)
+                               : pair_product<fp4::kMx, __half>(a, b, out, K, sm_count, status_word, pdl, stream);
 }
 
 }  // namespace lbl

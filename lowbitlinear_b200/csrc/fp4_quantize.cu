@@ -7,7 +7,9 @@
 // Both are bound by HBM: a value is read (or written) once in 2 or 4 bytes, and 0.53 (MXFP4) or 0.56
 // (NVFP4) bytes per value go the other way.  A thread owns sixteen neighbouring columns: one NVFP4
 // block, or half of an MXFP4 block whose other half sits in the neighbouring lane, so the largest
-// magnitude takes at most one shuffle; four scale bytes meet by shuffles and leave as one word.
+// magnitude takes at most one shuffle; four scale bytes meet by shuffles and leave as one word.  Rows are read and
+// written in 32-byte pieces per lane; rows that do not start on 16 bytes go through shared memory, where a warp
+// turns its 512 neighbouring columns from "a lane, one column after the other" to sixteen per lane.
 #include "fp4_common.cuh"
 #include "kernels.h"
 
@@ -15,6 +17,7 @@ namespace lbl {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kWarpCols = 512;  // columns of a row that one warp handles
 
 // One thread per (row, sixteen columns); rows are padded to whole scale tiles, so that every byte of
 // the scale buffer is written (zero where there is no value).
@@ -22,7 +25,7 @@ template <typename T, int kFormat>
 __global__ void __launch_bounds__(kThreads)
     fp4_quantize_kernel(const T* __restrict__ x, int64_t row_stride, const float* __restrict__ factor,
                         uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int64_t rows, int64_t cols,
-                        int units, bool vector_ok) {
+                        int units, int access) {
   pdl_allow_next_kernel();
   const int lane = threadIdx.x & 31;
   const int64_t row = static_cast<int64_t>(blockIdx.y) * blockDim.y + threadIdx.y;
@@ -35,8 +38,21 @@ __global__ void __launch_bounds__(kThreads)
 
   fp4::Sixteen<T> v;
   const T* src = x + row * row_stride + static_cast<int64_t>(unit) * 16;
-  if (vector_ok && valid == 16) {
-    v.load_vector(src);
+  if (access == fp4::kRowsAny) {
+    extern __shared__ __align__(32) uint8_t turned[];
+    T* mine = reinterpret_cast<T*>(turned) + (threadIdx.y * blockDim.x + threadIdx.x) / 32 * kWarpCols;
+    const int64_t first = static_cast<int64_t>(unit - lane) * 16;
+    const T* line = x + row * row_stride + first;
+    const int64_t end = row < rows ? cols - first : 0;
+#pragma unroll
+    for (int i = 0; i < kWarpCols / 32; ++i) {
+      const int c = i * 32 + lane;
+      mine[c] = c < end ? line[c] : static_cast<T>(0.0f);
+    }
+    __syncwarp();
+    v.load_vector(mine + lane * 16, fp4::kRows16);
+  } else if (valid == 16) {
+    v.load_vector(src, access);
   } else {
     v.load_masked(src, valid);
   }
@@ -88,60 +104,74 @@ template <typename T, int kFormat>
 __global__ void __launch_bounds__(kThreads)
     fp4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                           const float* __restrict__ factor, T* __restrict__ out, int64_t rows, int64_t cols,
-                          bool vector_ok) {
+                          int access) {
+  const int lane = threadIdx.x & 31;
   const int64_t row = static_cast<int64_t>(blockIdx.y) * blockDim.y + threadIdx.y;
-  const int unit = blockIdx.x * blockDim.x + threadIdx.x;
+  const int unit = blockIdx.x * blockDim.x + threadIdx.x;  // blockDim.x is a multiple of 32: a warp has one row
   const int64_t first = static_cast<int64_t>(unit) * 16;
-  if (row >= rows || first >= cols) return;
+  if (row >= rows) return;
   const int64_t pitch = fp4::code_pitch(cols);
   const int64_t tiles = fp4::scale_tiles(cols, kFormat);
-  const uint2 raw = __ldg(reinterpret_cast<const uint2*>(codes + row * pitch + unit * 8));
-  constexpr int kSpan = kFormat == fp4::kMx ? 2 : 1;
-  const int block = unit / kSpan;
-  const uint32_t byte = __ldg(scales + fp4::scale_word_offset(row, block >> 2, tiles) + (block & 3));
-  float g = 1.0f;
-  if constexpr (kFormat == fp4::kNv) g = factor == nullptr ? 1.0f : __ldg(factor);
-  const float step = fp4::step_of<kFormat>(byte, g);
   float v[16];
-  uint32_t pairs[4];
+  if (first < cols) {
+    const uint2 raw = __ldg(reinterpret_cast<const uint2*>(codes + row * pitch + static_cast<int64_t>(unit) * 8));
+    constexpr int kSpan = kFormat == fp4::kMx ? 2 : 1;
+    const int block = unit / kSpan;
+    const uint32_t byte = __ldg(scales + fp4::scale_word_offset(row, block >> 2, tiles) + (block & 3));
+    float g = 1.0f;
+    if constexpr (kFormat == fp4::kNv) g = factor == nullptr ? 1.0f : __ldg(factor);
+    const float step = fp4::step_of<kFormat>(byte, g);
+    uint32_t pairs[4];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    fp4::eight_values(h == 0 ? raw.x : raw.y, pairs);
+    for (int h = 0; h < 2; ++h) {
+      fp4::eight_values(h == 0 ? raw.x : raw.y, pairs);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = fp4::pair_to_float<__half>(pairs[i]);
-      v[h * 8 + 2 * i] = f.x * step;
-      v[h * 8 + 2 * i + 1] = f.y * step;
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = fp4::pair_to_float<__half>(pairs[i]);
+        v[h * 8 + 2 * i] = f.x * step;
+        v[h * 8 + 2 * i + 1] = f.y * step;
+      }
     }
   }
   T* dst = out + row * cols + first;
-  if (vector_ok && first + 16 <= cols) {
-    if constexpr (sizeof(T) == 4) {
+  if (access == fp4::kRowsAny) {
+    extern __shared__ __align__(32) uint8_t turned[];
+    T* mine = reinterpret_cast<T*>(turned) + (threadIdx.y * blockDim.x + threadIdx.x) / 32 * kWarpCols;
+    if (first < cols) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        reinterpret_cast<float4*>(dst)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-      }
-    } else {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint4 q;
-        q.x = two_rounded<T>(v[8 * h], v[8 * h + 1]);
-        q.y = two_rounded<T>(v[8 * h + 2], v[8 * h + 3]);
-        q.z = two_rounded<T>(v[8 * h + 4], v[8 * h + 5]);
-        q.w = two_rounded<T>(v[8 * h + 6], v[8 * h + 7]);
-        reinterpret_cast<uint4*>(dst)[h] = q;
-      }
+      for (int i = 0; i < 16; ++i) mine[lane * 16 + i] = static_cast<T>(v[i]);
     }
-  } else {
+    __syncwarp();
+    const int64_t line = static_cast<int64_t>(unit - lane) * 16;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      if (first + i < cols) {
+    for (int i = 0; i < kWarpCols / 32; ++i) {
+      const int c = i * 32 + lane;
+      if (line + c < cols) out[row * cols + line + c] = mine[c];
+    }
+  } else if (first + 16 <= cols) {
+    uint32_t w[8];
+#pragma unroll
+    for (int piece = 0; piece < static_cast<int>(sizeof(T)) / 2; ++piece) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
         if constexpr (sizeof(T) == 4) {
-          dst[i] = v[i];
+          w[i] = __float_as_uint(v[piece * 8 + i]);
         } else {
-          dst[i] = static_cast<T>(v[i]);
+          w[i] = two_rounded<T>(v[2 * i], v[2 * i + 1]);
         }
       }
+      if (access == fp4::kRows32) {
+        fp4::store_32_bytes(dst + piece * 8, w);
+      } else {
+        uint4* to = reinterpret_cast<uint4*>(dst + piece * 8);
+        to[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        to[1] = make_uint4(w[4], w[5], w[6], w[7]);
+      }
+    }
+  } else if (first < cols) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if (first + i < cols) dst[i] = static_cast<T>(v[i]);
     }
   }
 }
@@ -154,7 +184,7 @@ dim3 block_for(int64_t units) {
   return dim3(32 * x, kThreads / (32 * x));
 }
 
-constexpr int64_t kRowsPerLaunch = 65535LL * 1;  // limit of the grid's y extent (at one row per CTA)
+constexpr int64_t kRowsPerLaunch = 65535 / 128 * 128;  // limit of the grid's y extent, in whole scale tiles
 
 template <typename T, int kFormat>
 cudaError_t quantize(const void* x, int64_t row_stride, const float* factor, uint8_t* codes, uint8_t* scales,
@@ -165,15 +195,15 @@ cudaError_t quantize(const void* x, int64_t row_stride, const float* factor, uin
   const int64_t blocks_x = (units + block.x - 1) / block.x;
   const int64_t padded = (rows + 127) / 128 * 128;
   if (blocks_x > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
-  const bool vector_ok = (row_stride * sizeof(T)) % 16 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
-  constexpr int64_t kStep = kRowsPerLaunch / 128 * 128;  // whole scale tiles
-  for (int64_t r0 = 0; r0 < padded; r0 += kStep) {
-    const int64_t here = rows - r0 < kStep ? rows - r0 : kStep;
+  const int access = fp4::row_access(x, row_stride * static_cast<int64_t>(sizeof(T)));
+  const size_t smem = access == fp4::kRowsAny ? kThreads / 32 * kWarpCols * sizeof(T) : 0;
+  for (int64_t r0 = 0; r0 < padded; r0 += kRowsPerLaunch) {
+    const int64_t here = rows - r0 < kRowsPerLaunch ? rows - r0 : kRowsPerLaunch;
     const int64_t here_padded = (here + 127) / 128 * 128;
     const dim3 grid(static_cast<unsigned>(blocks_x), static_cast<unsigned>((here_padded + block.y - 1) / block.y));
-    fp4_quantize_kernel<T, kFormat><<<grid, block, 0, stream>>>(
+    fp4_quantize_kernel<T, kFormat><<<grid, block, smem, stream>>>(
         static_cast<const T*>(x) + r0 * row_stride, row_stride, factor, codes + r0 * fp4::code_pitch(cols),
-        scales + r0 / 128 * tiles * 512, here, cols, static_cast<int>(units), vector_ok);
+        scales + r0 / 128 * tiles * 512, here, cols, static_cast<int>(units), access);
     const cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess) return err;
   }
@@ -188,14 +218,14 @@ cudaError_t dequantize(const uint8_t* codes, const uint8_t* scales, const float*
   const dim3 block = block_for(units);
   const int64_t blocks_x = (units + block.x - 1) / block.x;
   if (blocks_x > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
-  const bool vector_ok = (cols * sizeof(T)) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
-  constexpr int64_t kStep = kRowsPerLaunch / 128 * 128;
-  for (int64_t r0 = 0; r0 < rows; r0 += kStep) {
-    const int64_t here = rows - r0 < kStep ? rows - r0 : kStep;
+  const int access = fp4::row_access(out, cols * static_cast<int64_t>(sizeof(T)));
+  const size_t smem = access == fp4::kRowsAny ? kThreads / 32 * kWarpCols * sizeof(T) : 0;
+  for (int64_t r0 = 0; r0 < rows; r0 += kRowsPerLaunch) {
+    const int64_t here = rows - r0 < kRowsPerLaunch ? rows - r0 : kRowsPerLaunch;
     const dim3 grid(static_cast<unsigned>(blocks_x), static_cast<unsigned>((here + block.y - 1) / block.y));
-    fp4_dequantize_kernel<T, kFormat><<<grid, block, 0, stream>>>(
+    fp4_dequantize_kernel<T, kFormat><<<grid, block, smem, stream>>>(
         codes + r0 * fp4::code_pitch(cols), scales + r0 / 128 * tiles * 512, factor, static_cast<T*>(out) + r0 * cols,
-        here, cols, vector_ok);
+        here, cols, access);
     const cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess) return err;
   }

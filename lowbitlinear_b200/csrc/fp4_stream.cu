@@ -39,7 +39,7 @@ struct StreamParams {
   int stages;
   int split;        // CTAs of a cluster, a power of two
   int split_shift;  // its logarithm
-  int x_vector;     // 16-byte loads of x allowed
+  int x_access;     // how rows of x may be read
   int receive_offset;  // where partial sums arrive in shared memory; 0: over the ring
   int* status;
 };
@@ -90,8 +90,8 @@ __device__ __forceinline__ void quantise_slice(const StreamParams& p, int k_begi
     const int valid = have ? min(16, max(0, p.cols - col)) : 0;
     const T* src = static_cast<const T*>(p.x) + row * p.x_stride + col;
     fp4::Sixteen<T> v;
-    if (valid == 16 && p.x_vector) {
-      v.load_vector(src);
+    if (valid == 16 && p.x_access != fp4::kRowsAny) {
+      v.load_vector(src, p.x_access);
     } else {
       v.load_masked(src, valid);
     }
@@ -376,7 +376,7 @@ cudaError_t launch(const Fp4Operand& w, const Fp4Operand& x, const void* raw, in
   params.split = split;
   params.split_shift = 0;
   while ((1 << params.split_shift) < split) ++params.split_shift;
-  params.x_vector = (raw_stride * 2) % 16 == 0 && reinterpret_cast<uintptr_t>(raw) % 16 == 0;
+  params.x_access = fp4::row_access(raw, raw_stride * 2);
   params.status = status;
   // Received partial sums have memory of their own while they are small, and lie over the ring otherwise.
   const bool own_memory = split > 1 && kQ <= 32;

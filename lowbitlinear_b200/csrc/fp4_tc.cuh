@@ -18,6 +18,10 @@ constexpr int kStageCols = 256;  // columns of K per pipeline stage
 constexpr int kRowBytes = kStageCols / 2;  // 128: one swizzle row
 constexpr int kMmaCols = 64;     // columns of K per MMA
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+
 // Untiled bulk copy of `bytes` (a multiple of 16) from global to shared memory.
 __device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
