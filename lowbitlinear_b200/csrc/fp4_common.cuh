@@ -36,8 +36,8 @@ __host__ __device__ constexpr int64_t scale_tiles(int64_t K, int format) {
   return (padded_cols(K) + tile_cols - 1) / tile_cols;
 }
 // Byte offset of the four scales of row r that belong to tile t along K.
-__device__ __forceinline__ int64_t scale_word_offset(int64_t r, int64_t t, int64_t tiles) {
-  return ((r >> 7) * tiles + t) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4;
+__device__ __forceinline__ int64_t scale_word_offset(int r, int t, int tiles) {
+  return (static_cast<int64_t>(r >> 7) * tiles + t) * 512 + ((r & 31) * 16 + ((r >> 5) & 3) * 4);
 }
 
 // Tensor factors outside this range would let a step or its reciprocal leave the normal FP32
@@ -50,10 +50,11 @@ __device__ __forceinline__ float e4m3_to_float(uint32_t byte) {
   return static_cast<float>(v);
 }
 
-// What one block needs to round its values.  `mul` is the reciprocal of the step.
+// What one block needs to round its values.  mul + mul_low is the reciprocal of the step, mul rounded down (MXFP4: mul
+// alone, exact).
 struct BlockStep {
   uint32_t byte;  // scale as stored
-  float step, mul;
+  float step, mul, mul_low;
   float limit;  // NVFP4: eight steps when the scale has saturated, infinity otherwise
   bool short_step;  // NVFP4: the step has the four bits of an E4M3 number (g is a power of two)
 };
@@ -82,7 +83,7 @@ __device__ __forceinline__ BlockStep mx_step(uint32_t amax_bits) {
   const bool bad = exponent == 255u;
   b.byte = bad ? 0xFFu : byte;
   b.mul = bad ? 0.0f : __uint_as_float((254u - byte) << 23);
-  b.step = 0.0f, b.limit = 0.0f, b.short_step = false;  // not used
+  b.step = 0.0f, b.mul_low = 0.0f, b.limit = 0.0f, b.short_step = false;  // not used
   return b;
 }
 
@@ -96,7 +97,7 @@ __device__ __forceinline__ TensorFactor tensor_factor(const float* factor) {
   f.g = factor == nullptr ? 1.0f : __ldg(factor);
   f.ok = factor_ok(f.g);
   f.six_g = f.ok ? 6.0f * f.g : 1.0f;
-  f.mul = __frcp_rn(f.six_g);
+  f.mul = __fdividef(1.0f, f.six_g);
   f.power_of_two = (__float_as_uint(f.g) & 0x7FFFFFu) == 0;
   return f;
 }
@@ -109,7 +110,8 @@ __device__ __forceinline__ BlockStep nv_step(uint32_t amax_bits, const TensorFac
   b.byte = bad ? 0x7Fu : byte;
   b.step = e4m3_to_float(byte) * f.g;
   const bool none = bad || byte == 0;  // a step of zero: every code is zero
-  b.mul = none ? 0.0f : __frcp_rn(b.step);
+  b.mul = none ? 0.0f : __frcp_rd(b.step);
+  b.mul_low = none ? 0.0f : fmaf(-b.mul, b.step, 1.0f) * b.mul;
   b.short_step = f.power_of_two;
   b.limit = byte >= 0x7Eu ? 8.0f * b.step : __uint_as_float(0x7F800000u);
   return b;
@@ -137,10 +139,11 @@ __device__ __forceinline__ uint32_t round_eight(const float (&x)[8], const Block
 #pragma unroll
     for (int i = 0; i < 8; ++i) q[i] = x[i] * b.mul;
   } else if (kHalfInput && b.short_step) {
-    // A number of at most eleven bits is either on a border (at most seven bits: three of the code's
-    // border, four of the step) or at least 2^-11 of it away, so the 17-bit quotient decides alone.
+    // The quotient to 47 bits, rounded once.  A number of at most eleven bits is either on a border (at most seven
+    // bits: three of the code's border, four of the step), and then comes out as the border itself, or at least 2^-11
+    // of it away.  Both products have the sign of x, zeros included.
 #pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = round_to_17_bits(x[i] * b.mul);
+    for (int i = 0; i < 8; ++i) q[i] = fmaf(x[i], b.mul, x[i] * b.mul_low);
   } else {
     // Only a saturated scale (8 steps < amax) makes the bound finite.  The sign of a zero is kept.
 #pragma unroll
@@ -272,7 +275,7 @@ struct SixteenHalves {
   __device__ __forceinline__ uint32_t amax_bits() const {
     uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+    for (int i = 0; i < 8; ++i) asm("max.u16x2 %0, %0, %1;" : "+r"(m) : "r"(w[i] & 0x7FFF7FFFu));
     const uint32_t top = max(m & 0xFFFFu, m >> 16);
     return __float_as_uint(pair_to_float<T>(top).x);
   }

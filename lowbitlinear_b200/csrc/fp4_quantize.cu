@@ -24,26 +24,23 @@ constexpr int kWarpCols = 512;  // columns of a row that one warp handles
 template <typename T, int kFormat>
 __global__ void __launch_bounds__(kThreads)
     fp4_quantize_kernel(const T* __restrict__ x, int64_t row_stride, const float* __restrict__ factor,
-                        uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int64_t rows, int64_t cols,
-                        int units, int access) {
+                        uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int rows, int cols, int pitch,
+                        int tiles, int access) {
   pdl_allow_next_kernel();
   const int lane = threadIdx.x & 31;
-  const int64_t row = static_cast<int64_t>(blockIdx.y) * blockDim.y + threadIdx.y;
+  const int row = blockIdx.y * blockDim.y + threadIdx.y;  // of this launch: fewer than 65536
   const int unit = blockIdx.x * blockDim.x + threadIdx.x;  // blockDim.x is a multiple of 32: a warp has one row
-  const int64_t padded_rows = (rows + 127) & ~static_cast<int64_t>(127);
-  if (row >= padded_rows) return;
-  const int64_t pitch = fp4::code_pitch(cols);
-  const int64_t tiles = fp4::scale_tiles(cols, kFormat);
-  const int valid = row < rows ? static_cast<int>(min(static_cast<int64_t>(16), max(static_cast<int64_t>(0), cols - static_cast<int64_t>(unit) * 16))) : 0;
+  if (row >= ((rows + 127) & ~127)) return;
+  const int first = unit * 16;
+  const int valid = row < rows ? min(16, cols - first) : 0;  // columns to read; below zero past the last one
 
   fp4::Sixteen<T> v;
-  const T* src = x + row * row_stride + static_cast<int64_t>(unit) * 16;
+  const T* src = x + (row * row_stride + first);
   if (access == fp4::kRowsAny) {
     extern __shared__ __align__(32) uint8_t turned[];
     T* mine = reinterpret_cast<T*>(turned) + (threadIdx.y * blockDim.x + threadIdx.x) / 32 * kWarpCols;
-    const int64_t first = static_cast<int64_t>(unit - lane) * 16;
-    const T* line = x + row * row_stride + first;
-    const int64_t end = row < rows ? cols - first : 0;
+    const T* line = src - lane * 16;
+    const int end = row < rows ? cols - first + lane * 16 : 0;
 #pragma unroll
     for (int i = 0; i < kWarpCols / 32; ++i) {
       const int c = i * 32 + lane;
@@ -71,7 +68,7 @@ __global__ void __launch_bounds__(kThreads)
   v.eight(1, part);
   out.y = fp4::round_eight<kFormat, sizeof(T) == 2>(part, step);
   const bool stored = row < rows && unit * 8 < pitch;
-  if (stored) *reinterpret_cast<uint2*>(codes + row * pitch + unit * 8) = out;
+  if (stored) *reinterpret_cast<uint2*>(codes + static_cast<int64_t>(row) * pitch + unit * 8) = out;
 
   // Blocks with no column (padding of the last tile, padding rows) have scale zero.
   uint32_t byte = stored ? step.byte : 0u;
@@ -103,18 +100,16 @@ __device__ __forceinline__ uint32_t two_rounded<__nv_bfloat16>(float a, float b)
 template <typename T, int kFormat>
 __global__ void __launch_bounds__(kThreads)
     fp4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                          const float* __restrict__ factor, T* __restrict__ out, int64_t rows, int64_t cols,
-                          int access) {
+                          const float* __restrict__ factor, T* __restrict__ out, int rows, int cols, int pitch,
+                          int tiles, int access) {
   const int lane = threadIdx.x & 31;
-  const int64_t row = static_cast<int64_t>(blockIdx.y) * blockDim.y + threadIdx.y;
+  const int row = blockIdx.y * blockDim.y + threadIdx.y;  // of this launch: fewer than 65536
   const int unit = blockIdx.x * blockDim.x + threadIdx.x;  // blockDim.x is a multiple of 32: a warp has one row
-  const int64_t first = static_cast<int64_t>(unit) * 16;
+  const int first = unit * 16;
   if (row >= rows) return;
-  const int64_t pitch = fp4::code_pitch(cols);
-  const int64_t tiles = fp4::scale_tiles(cols, kFormat);
   float v[16];
   if (first < cols) {
-    const uint2 raw = __ldg(reinterpret_cast<const uint2*>(codes + row * pitch + static_cast<int64_t>(unit) * 8));
+    const uint2 raw = __ldg(reinterpret_cast<const uint2*>(codes + static_cast<int64_t>(row) * pitch + unit * 8));
     constexpr int kSpan = kFormat == fp4::kMx ? 2 : 1;
     const int block = unit / kSpan;
     const uint32_t byte = __ldg(scales + fp4::scale_word_offset(row, block >> 2, tiles) + (block & 3));
@@ -133,7 +128,7 @@ __global__ void __launch_bounds__(kThreads)
       }
     }
   }
-  T* dst = out + row * cols + first;
+  T* dst = out + (static_cast<int64_t>(row) * cols + first);
   if (access == fp4::kRowsAny) {
     extern __shared__ __align__(32) uint8_t turned[];
     T* mine = reinterpret_cast<T*>(turned) + (threadIdx.y * blockDim.x + threadIdx.x) / 32 * kWarpCols;
@@ -142,11 +137,12 @@ __global__ void __launch_bounds__(kThreads)
       for (int i = 0; i < 16; ++i) mine[lane * 16 + i] = static_cast<T>(v[i]);
     }
     __syncwarp();
-    const int64_t line = static_cast<int64_t>(unit - lane) * 16;
+    T* line = dst - lane * 16;
+    const int end = cols - first + lane * 16;
 #pragma unroll
     for (int i = 0; i < kWarpCols / 32; ++i) {
       const int c = i * 32 + lane;
-      if (line + c < cols) out[row * cols + line + c] = mine[c];
+      if (c < end) line[c] = mine[c];
     }
   } else if (first + 16 <= cols) {
     uint32_t w[8];
@@ -203,7 +199,8 @@ cudaError_t quantize(const void* x, int64_t row_stride, const float* factor, uin
     const dim3 grid(static_cast<unsigned>(blocks_x), static_cast<unsigned>((here_padded + block.y - 1) / block.y));
     fp4_quantize_kernel<T, kFormat><<<grid, block, smem, stream>>>(
         static_cast<const T*>(x) + r0 * row_stride, row_stride, factor, codes + r0 * fp4::code_pitch(cols),
-        scales + r0 / 128 * tiles * 512, here, cols, static_cast<int>(units), access);
+        scales + r0 / 128 * tiles * 512, static_cast<int>(here), static_cast<int>(cols),
+        static_cast<int>(fp4::code_pitch(cols)), static_cast<int>(tiles), access);
     const cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess) return err;
   }
@@ -225,7 +222,8 @@ cudaError_t dequantize(const uint8_t* codes, const uint8_t* scales, const float*
     const dim3 grid(static_cast<unsigned>(blocks_x), static_cast<unsigned>((here + block.y - 1) / block.y));
     fp4_dequantize_kernel<T, kFormat><<<grid, block, smem, stream>>>(
         codes + r0 * fp4::code_pitch(cols), scales + r0 / 128 * tiles * 512, factor, static_cast<T*>(out) + r0 * cols,
-        here, cols, access);
+        static_cast<int>(here), static_cast<int>(cols), static_cast<int>(fp4::code_pitch(cols)), static_cast<int>(tiles),
+        access);
     const cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess) return err;
   }
