@@ -27,6 +27,7 @@ inference: no gradients are recorded.
 """
 import torch
 
+from . import _ops
 from .quantization import _row_chunks, _validate_matrix
 
 # format -> (code of the C ABI, columns per block)
@@ -216,8 +217,6 @@ def quantize_fp4(x, format="mxfp4", tensor_scale=None):
         rows, k = x.shape
         verdict = _remember(key, (x.is_cuda, rows, k, code_columns(k), scale_shape(rows, k, format), FORMATS[format][0]))
     if verdict[0]:
-        from . import _ops
-
         return _ops.fp4_quantize(x, tensor_scale, verdict)
     rows, k = x.shape
     codes = torch.empty((rows, code_columns(k)), dtype=torch.uint8)
@@ -246,8 +245,6 @@ def dequantize_fp4(codes, scales, in_features=None, format="mxfp4", tensor_scale
         _validate_factor(tensor_scale, "tensor_scale", format, codes.device)
         verdict = _remember(key, (codes.is_cuda, rows, k, FORMATS[format][0], dtype))
     if verdict[0]:
-        from . import _ops
-
         return _ops.fp4_dequantize(codes, scales, tensor_scale, verdict)
     return _operand_values(codes, scales, format, tensor_scale)[:, :verdict[2]].to(dtype).contiguous()
 
@@ -280,8 +277,6 @@ def matmul_fp4(a_codes, a_scales, b_codes, b_scales, format="mxfp4", a_scale=Non
         _validate_factor(b_scale, "b_scale", format, a_codes.device)
         verdict = _remember(key, (a_codes.is_cuda, m, n, k, FORMATS[format][0], dtype))
     if verdict[0]:
-        from . import _ops
-
         return _ops.fp4_matmul(a_codes, a_scales, b_codes, b_scales, a_scale, b_scale, verdict)
     y = _operand_values(a_codes, a_scales, format, None) @ _operand_values(b_codes, b_scales, format, None).T
     for factor in (a_scale, b_scale):
@@ -315,13 +310,9 @@ def linear_fp4(x, codes, scales, format="mxfp4", tensor_scale=None, input_scale=
         _validate_factor(input_scale, "input_scale", format, x.device)
         need = 0
         if x.is_cuda:
-            from . import _ops
-
-            need = _ops.fp4_workspace_bytes(m, n, k, format)
+                need = _ops.fp4_workspace_bytes(m, n, k, format)
         verdict = _remember(key, (x.is_cuda, m, n, k, FORMATS[format][0], need))
     if verdict[0]:
-        from . import _ops
-
         return _ops.fp4_linear(x, codes, scales, tensor_scale, input_scale, verdict)
     x_codes, x_scales = quantize_fp4(x, format, input_scale)
     return matmul_fp4(x_codes, x_scales, codes, scales, format, input_scale, tensor_scale, x.dtype)
