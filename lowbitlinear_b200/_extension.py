@@ -75,6 +75,10 @@ def load_cuda_extension(*, required=False):
 
     _native = _ops.bind(str(path))
     _ops.register_operators(_native)
+    if (path.parent / "_binding.so").is_file():  # built together with the library
+        from . import _binding
+
+        _ops.set_binding(_binding)
     _loaded_library = path
     return True
 

@@ -514,7 +514,18 @@ def dequantize(packed_w, scales, zeros, in_features=None, dtype=torch.float16, g
     return weight
 
 
+FP4_FORMATS = {"mxfp4": 0, "nvfp4": 1}
 FP4_TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+binding = None  # the module _binding (csrc/binding.cpp): the same calls without ctypes
+
+
+def set_binding(module):
+    """Hand the library's FP4 entry points to the torch binding and use it from now on."""
+    global binding
+    module.bind(*(ctypes.cast(f, ctypes.c_void_p).value
+                  for f in (_lib.lbl_fp4_quantize, _lib.lbl_fp4_dequantize, _lib.lbl_fp4_matmul,
+                            _lib.lbl_fp4_linear_workspace_bytes, _lib.lbl_fp4_linear)))
+    binding = module
 
 
 def _fp4_library():
@@ -529,75 +540,63 @@ def _pointer(tensor):
     return None if tensor is None else tensor.data_ptr()
 
 
-def fp4_workspace_bytes(m, n, k, format):
-    """Scratch ``fp4_linear`` needs (``lbl_fp4_linear_workspace_bytes``)."""
-    return _fp4_library().lbl_fp4_linear_workspace_bytes(m, n, k, {"mxfp4": 0, "nvfp4": 1}[format])
+def _contiguous_rows(x):
+    return x if x.stride(1) == 1 and x.stride(0) >= 0 else x.contiguous()
 
 
-def fp4_quantize(x, tensor_scale, verdict):
-    """Microscaled quantisation of a CUDA matrix in one kernel.  ``microscaling.quantize_fp4`` has checked
-    the arguments and passes what it found.  Rows may be strided; other layouts are made contiguous."""
-    lib = _lib or _fp4_library()
-    _, rows, k, columns, scale_shape, format = verdict
-    stride, inner = x.stride()
-    if inner != 1 or stride < 0:
-        x = x.contiguous()
-        stride = k
-    device = x.device
-    codes = x.new_empty((rows, columns), dtype=torch.uint8)
-    scales = x.new_empty(scale_shape, dtype=torch.uint8)
-    rc = lib.lbl_fp4_quantize(x.data_ptr(), FP4_TYPES[x.dtype], rows, k, stride, format, _pointer(tensor_scale),
-                              codes.data_ptr(), scales.data_ptr(), device.index, _raw_stream(device))
-    if rc:
-        _check(rc)
+def fp4_quantize(x, format, tensor_scale=None):
+    """Microscaled quantisation of a CUDA matrix in one kernel (``microscaling.quantize_fp4``, which
+    checks the arguments).  Rows may be strided; other layouts are made contiguous first."""
+    lib = _fp4_library()
+    x = _contiguous_rows(x)
+    rows, k = x.shape
+    columns = (k + 31) // 32 * 16
+    blocks = columns * 2 // (16 if format == "nvfp4" else 32)
+    codes = torch.empty((rows, columns), dtype=torch.uint8, device=x.device)
+    scales = torch.empty(((rows + 127) // 128, (blocks + 3) // 4, 32, 4, 4), dtype=torch.uint8, device=x.device)
+    _check(lib.lbl_fp4_quantize(x.data_ptr(), FP4_TYPES[x.dtype], rows, k, x.stride(0), FP4_FORMATS[format],
+                                _pointer(tensor_scale), codes.data_ptr(), scales.data_ptr(), x.device.index,
+                                _raw_stream(x.device)))
     return codes, scales
 
 
-def fp4_dequantize(codes, scales, tensor_scale, verdict):
+def fp4_dequantize(codes, scales, in_features, format, tensor_scale=None, dtype=torch.float16):
     """The inverse (``microscaling.dequantize_fp4``)."""
-    lib = _lib or _fp4_library()
-    _, rows, k, format, dtype = verdict
-    device = codes.device
-    out = codes.new_empty((rows, k), dtype=dtype)
-    rc = lib.lbl_fp4_dequantize(codes.data_ptr(), scales.data_ptr(), rows, k, format, _pointer(tensor_scale),
-                                out.data_ptr(), FP4_TYPES[dtype], device.index, _raw_stream(device))
-    if rc:
-        _check(rc)
+    lib = _fp4_library()
+    rows = codes.size(0)
+    out = torch.empty((rows, in_features), dtype=dtype, device=codes.device)
+    _check(lib.lbl_fp4_dequantize(codes.data_ptr(), scales.data_ptr(), rows, in_features, FP4_FORMATS[format],
+                                  _pointer(tensor_scale), out.data_ptr(), FP4_TYPES[dtype], codes.device.index,
+                                  _raw_stream(codes.device)))
     return out
 
 
-def fp4_matmul(a_codes, a_scales, b_codes, b_scales, a_scale, b_scale, verdict):
+def fp4_matmul(a_codes, a_scales, b_codes, b_scales, format, a_scale=None, b_scale=None, dtype=torch.float16):
     """Product of two quantised operands (``microscaling.matmul_fp4``)."""
-    lib = _lib or _fp4_library()
-    _, m, n, k, format, dtype = verdict
-    device = a_codes.device
-    out = a_codes.new_empty((m, n), dtype=dtype)
-    rc = lib.lbl_fp4_matmul(a_codes.data_ptr(), a_scales.data_ptr(), _pointer(a_scale), b_codes.data_ptr(),
-                            b_scales.data_ptr(), _pointer(b_scale), out.data_ptr(), m, n, k, format, FP4_TYPES[dtype],
-                            _flags, device.index, _raw_stream(device))
-    if rc:
-        _check(rc)
+    lib = _fp4_library()
+    m, n, k = a_codes.size(0), b_codes.size(0), a_codes.size(1) * 2
+    out = torch.empty((m, n), dtype=dtype, device=a_codes.device)
+    _check(lib.lbl_fp4_matmul(a_codes.data_ptr(), a_scales.data_ptr(), _pointer(a_scale), b_codes.data_ptr(),
+                              b_scales.data_ptr(), _pointer(b_scale), out.data_ptr(), m, n, k, FP4_FORMATS[format],
+                              FP4_TYPES[dtype], _flags, a_codes.device.index, _raw_stream(a_codes.device)))
     return out
 
 
-def fp4_linear(x, codes, scales, tensor_scale, input_scale, verdict):
+def fp4_linear(x, codes, scales, format, tensor_scale=None, input_scale=None):
     """Linear layer with quantised weights and activations (``microscaling.linear_fp4``).  The scratch
     for the quantised activations is allocated per call, so calls on different streams, and graphs
     captured from them, share nothing."""
-    lib = _lib or _fp4_library()
-    _, m, n, k, format, need = verdict
-    stride, inner = x.stride()
-    if inner != 1 or stride < 0:
-        x = x.contiguous()
-        stride = k
-    device = x.device
-    y = x.new_empty((m, n))
-    scratch = codes.new_empty(need) if need else None
-    rc = lib.lbl_fp4_linear(x.data_ptr(), FP4_TYPES[x.dtype], stride, _pointer(input_scale), codes.data_ptr(),
-                            scales.data_ptr(), _pointer(tensor_scale), y.data_ptr(), m, n, k, format,
-                            _pointer(scratch), need, _flags, device.index, _raw_stream(device))
-    if rc:
-        _check(rc)
+    lib = _fp4_library()
+    x = _contiguous_rows(x)
+    m, k = x.shape
+    n = codes.size(0)
+    kind = FP4_FORMATS[format]
+    y = torch.empty((m, n), dtype=x.dtype, device=x.device)
+    need = lib.lbl_fp4_linear_workspace_bytes(m, n, k, kind)
+    scratch = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    _check(lib.lbl_fp4_linear(x.data_ptr(), FP4_TYPES[x.dtype], x.stride(0), _pointer(input_scale), codes.data_ptr(),
+                              scales.data_ptr(), _pointer(tensor_scale), y.data_ptr(), m, n, k, kind,
+                              _pointer(scratch), need, _flags, x.device.index, _raw_stream(x.device)))
     return y
 
 

@@ -168,59 +168,28 @@ def _operand_values(codes, scales, format, factor):
 
 # ---- operators -----------------------------------------------------------------------------------
 #
-# At decode sizes the checks of a call cost more host time than its kernel runs, so a set of arguments that
-# passed once is recognised by everything the checks look at (types, shapes, dtypes, devices, strides
-# where they matter), never by its contents or identity: equal keys mean an equal verdict.  The verdict
-# holds the sizes and codes that the native call needs.
-
-_passed = {}
-_MOST_VERDICTS = 4096
-
-
-def _remember(key, verdict):
-    if key is not None:
-        if len(_passed) >= _MOST_VERDICTS:
-            _passed.clear()
-        _passed[key] = verdict
-    return verdict
-
-
-def _known(key):
-    try:
-        return _passed.get(key)
-    except TypeError:  # an argument that cannot be hashed: the checks name it
-        return None
-
-
-def _factor_key(factor):
-    return None if factor is None else (type(factor), factor.dtype, factor.shape, factor.device)
-
-
-def _operand_key(codes, scales):
-    return (type(codes), codes.dtype, codes.shape, codes.device, codes.is_contiguous(),
-            type(scales), scales.dtype, scales.shape, scales.device, scales.is_contiguous())
+# At decode sizes the checks of a call cost more host time than its kernel runs.  The torch binding looks at the
+# same things without the interpreter and answers None to whatever is not a plain call on CUDA tensors; the
+# checks here then say what is wrong, or the call goes its other way.
 
 
 def quantize_fp4(x, format="mxfp4", tensor_scale=None):
     """Quantise ``x`` ``[R, K]`` (FP16, BF16 or FP32): ``(codes, scales)`` in the layout above.
 
     ``tensor_scale`` is the FP32 factor ``g`` of nvfp4, one value on ``x``'s device."""
-    try:
-        key = ("quantize", type(x), x.dtype, x.shape, x.device, format, _factor_key(tensor_scale))
-    except AttributeError:
-        key = None
-    verdict = _known(key)
-    if verdict is None:
-        _validate_matrix(x, "x", _FLOAT_TYPES)
-        _validate_format(format)
-        _validate_factor(tensor_scale, "tensor_scale", format, x.device)
-        rows, k = x.shape
-        verdict = _remember(key, (x.is_cuda, rows, k, code_columns(k), scale_shape(rows, k, format), FORMATS[format][0]))
-    if verdict[0]:
-        return _ops.fp4_quantize(x, tensor_scale, verdict)
+    if _ops.binding is not None:
+        result = _ops.binding.quantize(x, format, tensor_scale)
+        if result is not None:
+            return result
+    _validate_matrix(x, "x", _FLOAT_TYPES)
+    _validate_format(format)
+    _validate_factor(tensor_scale, "tensor_scale", format, x.device)
+    if x.is_cuda:
+        return _ops.fp4_quantize(x, format, tensor_scale)
     rows, k = x.shape
+    _, block = FORMATS[format]
     codes = torch.empty((rows, code_columns(k)), dtype=torch.uint8)
-    scales = torch.empty((rows, code_columns(k) * 2 // FORMATS[format][1]), dtype=torch.uint8)
+    scales = torch.empty((rows, code_columns(k) * 2 // block), dtype=torch.uint8)
     for r0, r1 in _row_chunks(rows, k):
         codes[r0:r1], scales[r0:r1] = _quantize_rows(x.detach()[r0:r1], format, tensor_scale)
     return codes, tile_scales(scales)
@@ -229,24 +198,20 @@ def quantize_fp4(x, format="mxfp4", tensor_scale=None):
 def dequantize_fp4(codes, scales, in_features=None, format="mxfp4", tensor_scale=None, dtype=torch.float16):
     """``code * step`` as ``[R, in_features]``, computed in FP32 and rounded once to ``dtype`` (FP16,
     BF16 or FP32).  ``in_features`` defaults to the padded column count."""
-    try:
-        key = ("dequantize", _operand_key(codes, scales), type(in_features), in_features, format,
-               _factor_key(tensor_scale), dtype)
-    except AttributeError:
-        key = None
-    verdict = _known(key)
-    if verdict is None:
-        _validate_format(format)
-        if dtype not in _FLOAT_TYPES:
-            raise TypeError("dtype must be FP16, BF16 or FP32")
-        _validate_matrix(codes, "codes", (torch.uint8,))
-        k = codes.shape[1] * 2 if in_features is None else in_features
-        rows = _validate_operand(codes, scales, format, k)
-        _validate_factor(tensor_scale, "tensor_scale", format, codes.device)
-        verdict = _remember(key, (codes.is_cuda, rows, k, FORMATS[format][0], dtype))
-    if verdict[0]:
-        return _ops.fp4_dequantize(codes, scales, tensor_scale, verdict)
-    return _operand_values(codes, scales, format, tensor_scale)[:, :verdict[2]].to(dtype).contiguous()
+    if _ops.binding is not None:
+        result = _ops.binding.dequantize(codes, scales, in_features, format, tensor_scale, dtype)
+        if result is not None:
+            return result
+    _validate_format(format)
+    if dtype not in _FLOAT_TYPES:
+        raise TypeError("dtype must be FP16, BF16 or FP32")
+    _validate_matrix(codes, "codes", (torch.uint8,))
+    k = codes.shape[1] * 2 if in_features is None else in_features
+    _validate_operand(codes, scales, format, k)
+    _validate_factor(tensor_scale, "tensor_scale", format, codes.device)
+    if codes.is_cuda:
+        return _ops.fp4_dequantize(codes, scales, k, format, tensor_scale, dtype)
+    return _operand_values(codes, scales, format, tensor_scale)[:, :k].to(dtype).contiguous()
 
 
 def matmul_fp4(a_codes, a_scales, b_codes, b_scales, format="mxfp4", a_scale=None, b_scale=None,
@@ -254,30 +219,26 @@ def matmul_fp4(a_codes, a_scales, b_codes, b_scales, format="mxfp4", a_scale=Non
     """``a . b^T`` of two quantised operands ``[Ra, K]`` and ``[Rb, K]``: ``[Ra, Rb]`` in ``dtype`` (FP16
     or BF16), FP32 sums, one rounding.  ``a_scale`` and ``b_scale`` are the operands' nvfp4 factors.
     What the codes past column K hold is multiplied too: they are zero as ``quantize_fp4`` writes them."""
-    try:
-        key = ("matmul", _operand_key(a_codes, a_scales), _operand_key(b_codes, b_scales), format,
-               _factor_key(a_scale), _factor_key(b_scale), dtype)
-    except AttributeError:
-        key = None
-    verdict = _known(key)
-    if verdict is None:
-        _validate_format(format)
-        if dtype not in _HALF_TYPES:
-            raise TypeError("dtype must be FP16 or BF16")
-        _validate_matrix(a_codes, "a_codes", (torch.uint8,))
-        k = a_codes.shape[1] * 2
-        m = _validate_operand(a_codes, a_scales, format, k, "a_")
-        _validate_matrix(b_codes, "b_codes", (torch.uint8,))
-        if b_codes.shape[1] != a_codes.shape[1]:
-            raise ValueError("a_codes and b_codes have incompatible K")
-        n = _validate_operand(b_codes, b_scales, format, k, "b_")
-        if a_codes.device != b_codes.device:
-            raise ValueError("All tensors must be on the same device")
-        _validate_factor(a_scale, "a_scale", format, a_codes.device)
-        _validate_factor(b_scale, "b_scale", format, a_codes.device)
-        verdict = _remember(key, (a_codes.is_cuda, m, n, k, FORMATS[format][0], dtype))
-    if verdict[0]:
-        return _ops.fp4_matmul(a_codes, a_scales, b_codes, b_scales, a_scale, b_scale, verdict)
+    if _ops.binding is not None:
+        result = _ops.binding.matmul(a_codes, a_scales, b_codes, b_scales, format, a_scale, b_scale, dtype, _ops._flags)
+        if result is not None:
+            return result
+    _validate_format(format)
+    if dtype not in _HALF_TYPES:
+        raise TypeError("dtype must be FP16 or BF16")
+    _validate_matrix(a_codes, "a_codes", (torch.uint8,))
+    k = a_codes.shape[1] * 2
+    _validate_operand(a_codes, a_scales, format, k, "a_")
+    _validate_matrix(b_codes, "b_codes", (torch.uint8,))
+    if b_codes.shape[1] != a_codes.shape[1]:
+        raise ValueError("a_codes and b_codes have incompatible K")
+    _validate_operand(b_codes, b_scales, format, k, "b_")
+    if a_codes.device != b_codes.device:
+        raise ValueError("All tensors must be on the same device")
+    _validate_factor(a_scale, "a_scale", format, a_codes.device)
+    _validate_factor(b_scale, "b_scale", format, a_codes.device)
+    if a_codes.is_cuda:
+        return _ops.fp4_matmul(a_codes, a_scales, b_codes, b_scales, format, a_scale, b_scale, dtype)
     y = _operand_values(a_codes, a_scales, format, None) @ _operand_values(b_codes, b_scales, format, None).T
     for factor in (a_scale, b_scale):
         if factor is not None:
@@ -290,30 +251,23 @@ def linear_fp4(x, codes, scales, format="mxfp4", tensor_scale=None, input_scale=
     weight ``codes`` / ``scales`` / ``tensor_scale`` ``[N, K]``: ``[M, N]`` in ``x``'s type.
 
     ``matmul_fp4(*quantize_fp4(x, format, input_scale), codes, scales, ...)`` in one call."""
-    try:
-        key = ("linear", type(x), x.dtype, x.shape, x.device, _operand_key(codes, scales), format,
-               _factor_key(tensor_scale), _factor_key(input_scale))
-    except AttributeError:
-        key = None
-    verdict = _known(key)
-    if verdict is None:
-        _validate_format(format)
-        _validate_matrix(x, "x", _HALF_TYPES)
-        _validate_matrix(codes, "codes", (torch.uint8,))
-        m, k = x.shape
-        if codes.shape[1] != code_columns(k):
-            raise ValueError("x and codes have incompatible K")
-        n = _validate_operand(codes, scales, format, k)
-        if x.device != codes.device:
-            raise ValueError("All tensors must be on the same device")
-        _validate_factor(tensor_scale, "tensor_scale", format, x.device)
-        _validate_factor(input_scale, "input_scale", format, x.device)
-        need = 0
-        if x.is_cuda:
-                need = _ops.fp4_workspace_bytes(m, n, k, format)
-        verdict = _remember(key, (x.is_cuda, m, n, k, FORMATS[format][0], need))
-    if verdict[0]:
-        return _ops.fp4_linear(x, codes, scales, tensor_scale, input_scale, verdict)
+    if _ops.binding is not None:
+        result = _ops.binding.linear(x, codes, scales, format, tensor_scale, input_scale, _ops._flags)
+        if result is not None:
+            return result
+    _validate_format(format)
+    _validate_matrix(x, "x", _HALF_TYPES)
+    _validate_matrix(codes, "codes", (torch.uint8,))
+    k = x.shape[1]
+    if codes.shape[1] != code_columns(k):
+        raise ValueError("x and codes have incompatible K")
+    _validate_operand(codes, scales, format, k)
+    if x.device != codes.device:
+        raise ValueError("All tensors must be on the same device")
+    _validate_factor(tensor_scale, "tensor_scale", format, x.device)
+    _validate_factor(input_scale, "input_scale", format, x.device)
+    if x.is_cuda:
+        return _ops.fp4_linear(x, codes, scales, format, tensor_scale, input_scale)
     x_codes, x_scales = quantize_fp4(x, format, input_scale)
     return matmul_fp4(x_codes, x_scales, codes, scales, format, input_scale, tensor_scale, x.dtype)
 

@@ -238,3 +238,40 @@ def test_empty_outputs_and_refusals(cuda_ops):
     with pytest.raises(RuntimeError, match="aligned"):
         matmul_fp4(shifted, scales, codes, scales)
     assert torch.equal(linear_fp4(x, codes, scales), torch.full((4, 4), 64.0, dtype=torch.float16, device=cuda_ops))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("m", [1, 40, 300])
+def test_both_bindings_make_the_same_calls(cuda_ops, fmt, m, monkeypatch):
+    """The torch binding and the ctypes path behind it: same bits, same refusals."""
+    from lowbitlinear_b200 import _ops
+
+    assert _ops.binding is not None, "csrc/binding.cpp was not built"
+    g = on(cuda_ops, factor_of(fmt, 0.02))
+    x = torch.randn(m, 200, device=cuda_ops).bfloat16()
+    weight = quantize_fp4(torch.randn(300, 200, device=cuda_ops), fmt)
+
+    def everything():
+        codes, scales = quantize_fp4(x, fmt, g)
+        outputs = [codes, scales, dequantize_fp4(codes, scales, 200, fmt, g, torch.float32),
+                   dequantize_fp4(codes, scales, format=fmt, tensor_scale=g),
+                   matmul_fp4(codes, scales, *weight, fmt, g, None, torch.bfloat16), linear_fp4(x, *weight, fmt, None, g)]
+        outputs.append(quantize_fp4(torch.nn.Parameter(x.float()), fmt, g)[0])
+        for bad, error in ((lambda: linear_fp4(x.double(), *weight, fmt), TypeError),
+                           (lambda: linear_fp4(x[:, :100], *weight, fmt), ValueError),
+                           (lambda: linear_fp4(x, weight[0], weight[1][:1], fmt), ValueError),
+                           (lambda: linear_fp4(x[:0], *weight, fmt), ValueError),
+                           (lambda: matmul_fp4(codes, scales, *weight, "fp4"), ValueError),
+                           (lambda: dequantize_fp4(codes, scales, True, fmt), ValueError),
+                           (lambda: dequantize_fp4(codes, scales, 1 << 70, fmt), ValueError),
+                           (lambda: dequantize_fp4(codes, scales, 200, fmt, dtype="float"), TypeError),
+                           (lambda: quantize_fp4(x, fmt, torch.ones(2, device=cuda_ops)), ValueError),
+                           (lambda: quantize_fp4(x, [], g), ValueError)):
+            with pytest.raises(error):
+                bad()
+        return outputs
+
+    with_binding = everything()
+    monkeypatch.setattr(_ops, "binding", None)
+    for a, b in zip(with_binding, everything()):
+        assert torch.equal(a, b) and a.dtype == b.dtype
