@@ -462,11 +462,11 @@ bool fp4_use_pair(int64_t M, int64_t N, int sm_count) {
 }
 
 int run_fp4_matmul(const lbl::Fp4Operand& a, const lbl::Fp4Operand& b, int64_t K, int format, void* out, int out_type,
-                   bool pdl, cudaStream_t stream, const DeviceInfo& info) {
+                   bool early_weight, cudaStream_t stream, const DeviceInfo& info) {
   const cudaError_t err =
       fp4_use_pair(a.rows, b.rows, info.sm_count)
-          ? lbl::launch_fp4_pair(a, b, format, out, out_type, K, info.sm_count, info.status_word, pdl, stream)
-          : lbl::launch_fp4_stream(a, b, format, out, out_type, K, info.sm_count, info.status_word, pdl, stream);
+          ? lbl::launch_fp4_pair(a, b, format, out, out_type, K, info.sm_count, info.status_word, stream)
+          : lbl::launch_fp4_stream(a, b, format, out, out_type, K, info.sm_count, info.status_word, early_weight, stream);
   if (err != cudaSuccess) return fail_cuda(err, "FP4 product launch");
   return LBL_OK;
 }
@@ -492,7 +492,8 @@ int lbl_fp4_quantize(const void* x, int x_type, int64_t rows, int64_t cols, int6
   if (!scope.ok()) return fail(LBL_ERR_CUDA, "cannot make device %d current", device);
   const cudaError_t err =
       lbl::launch_fp4_quantize(x, x_type, row_stride, format, factor, static_cast<uint8_t*>(codes),
-                               static_cast<uint8_t*>(scales), rows, cols, static_cast<cudaStream_t>(stream));
+                               static_cast<uint8_t*>(scales), rows, cols, /*early_successor=*/false,
+                               static_cast<cudaStream_t>(stream));
   if (err != cudaSuccess) return fail_cuda(err, "FP4 quantise launch");
   return LBL_OK;
 }
@@ -585,11 +586,13 @@ int lbl_fp4_linear(const void* x, int x_type, int64_t x_row_stride, const float*
   }
   uint8_t* codes = static_cast<uint8_t*>(workspace);
   uint8_t* scales = codes + fp4_code_bytes(M, K);  // a multiple of 16 bytes
-  const cudaError_t err = lbl::launch_fp4_quantize(x, x_type, x_row_stride, format, x_factor, codes, scales, M, K, cu_stream);
+  const cudaError_t err = lbl::launch_fp4_quantize(x, x_type, x_row_stride, format, x_factor, codes, scales, M, K,
+                                                    /*early_successor=*/true, cu_stream);
   if (err != cudaSuccess) return fail_cuda(err, "FP4 quantise launch");
   const lbl::Fp4Operand a = {codes, scales, x_factor, M};
-  // The product starts beside the quantiser and waits for it before it touches the codes.
-  return run_fp4_matmul(a, b, K, format, y, x_type, /*pdl=*/true, cu_stream, info);
+  // The product fetches the weight beside the quantiser, which started after everything before it, and waits for it
+  // before it touches the codes.
+  return run_fp4_matmul(a, b, K, format, y, x_type, /*early_weight=*/true, cu_stream, info);
 }
 
 int lbl_device_status(int device, int* status) {

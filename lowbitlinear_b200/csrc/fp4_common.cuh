@@ -179,6 +179,18 @@ __device__ __forceinline__ float step_of(uint32_t byte, float g) {
 }
 
 // ---- sixteen neighbouring activations or weights as they lie in memory -------------------------
+// Every FP4 kernel is launched with programmatic dependent launch: its set-up overlaps the end of the kernel in front,
+// and it reads and writes global memory only after griddepcontrol.wait, when that kernel is complete
+// (LBL_FLAG_PDL: the weight is fetched before).  Every CTA waits, so a kernel ends after its predecessor, and it lets
+// its successor start only after the wait, so whatever ran two kernels earlier is complete by then.  The
+// quantiser of weights and the dequantiser never let a successor start early.
+inline cudaLaunchAttribute programmatic_launch() {
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  return attr;
+}
+
 // How the rows of a matrix may be read or written, by the alignment of its base and pitch.
 constexpr int kRows32 = 2;  // 32-byte accesses
 constexpr int kRows16 = 1;  // 16-byte accesses

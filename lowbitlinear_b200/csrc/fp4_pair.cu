@@ -215,10 +215,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   cluster_sync_all();
   tc_fence_after_sync();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&bars.tmem_base);
+  pdl_wait_for_previous_kernel();
   pdl_allow_next_kernel();
 
   if (warp == 0) {
-    pdl_wait_for_previous_kernel();
     const uint32_t full = map_to_cta(smem_addr(&bars.full[0]), leader);
     int i = 0;  // stages since the start
     for (int t = first_tile; t < tiles; t += tile_step) {
@@ -274,7 +274,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else if constexpr (!kSplit) {
-    pdl_wait_for_previous_kernel();
     const float alpha = product_factor(p.factor_a, p.factor_b);
     const uint32_t acc_free = map_to_cta(smem_addr(&bars.acc_free), leader);
     const int quarter = warp & 3;
@@ -312,7 +311,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t acc = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     bool ok = false;
     if (warp >= 2) {
-      pdl_wait_for_previous_kernel();
       ok = warp_wait(&bars.acc_full, 0, abort_flag, p.status, kStatusPairWait + 4);
       tc_fence_after_sync();
     }
@@ -388,7 +386,7 @@ bool encode_scales(CUtensorMap* map, const uint8_t* scales, int64_t rows, int64_
 }
 
 template <int kFormat, bool kSplit, typename T>
-cudaError_t launch(const Fp4Operand& a, const Fp4Operand& b, void* out, int64_t K, int sm_count, int* status, bool pdl,
+cudaError_t launch(const Fp4Operand& a, const Fp4Operand& b, void* out, int64_t K, int sm_count, int* status,
                    cudaStream_t stream) {
   using Tile = PairTile<kFormat>;
   const int64_t pitch = fp4::code_pitch(K);
@@ -436,32 +434,31 @@ cudaError_t launch(const Fp4Operand& a, const Fp4Operand& b, void* out, int64_t 
   attr[0].val.clusterDim.x = kSplit ? 4 : 2;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  attr[1] = fp4::programmatic_launch();
   cfg.attrs = attr;
-  cfg.numAttrs = pdl ? 2 : 1;
+  cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, kernel, map_a, map_b, map_sa, map_sb, params);
 }
 
 template <int kFormat, typename T>
 cudaError_t pair_product(const Fp4Operand& a, const Fp4Operand& b, void* out, int64_t K, int sm_count, int* status,
-                         bool pdl, cudaStream_t stream) {
+                         cudaStream_t stream) {
   const int64_t tiles = ((a.rows + kRowsPair - 1) / kRowsPair) * ((b.rows + kRowsPair - 1) / kRowsPair);
   const bool split = 2 * tiles <= sm_count / 2 && fp4::padded_cols(K) > 3 * kStageCols;
-  return split ? launch<kFormat, true, T>(a, b, out, K, sm_count, status, pdl, stream)
-               : launch<kFormat, false, T>(a, b, out, K, sm_count, status, pdl, stream);
+  return split ? launch<kFormat, true, T>(a, b, out, K, sm_count, status, stream)
+               : launch<kFormat, false, T>(a, b, out, K, sm_count, status, stream);
 }
 
 }  // namespace
 
 cudaError_t launch_fp4_pair(const Fp4Operand& a, const Fp4Operand& b, int format, void* out, int out_type, int64_t K,
-                            int sm_count, int* status_word, bool pdl, cudaStream_t stream) {
+                            int sm_count, int* status_word, cudaStream_t stream) {
   if (format == fp4::kNv) {
-    return out_type == kTypeBf16 ? pair_product<fp4::kNv, __nv_bfloat16>(a, b, out, K, sm_count, status_word, pdl, stream)
-                                 : pair_product<fp4::kNv, __half>(a, b, out, K, sm_count, status_word, pdl, stream);
+    return out_type == kTypeBf16 ? pair_product<fp4::kNv, __nv_bfloat16>(a, b, out, K, sm_count, status_word, stream)
+                                 : pair_product<fp4::kNv, __half>(a, b, out, K, sm_count, status_word, stream);
   }
-  return out_type == kTypeBf16 ? pair_product<fp4::kMx, __nv_bfloat16>(a, b, out, K, sm_count, status_word, pdl, stream)
-                               : pair_product<fp4::kMx, __half>(a, b, out, K, sm_count, status_word, pdl, stream);
+  return out_type == kTypeBf16 ? pair_product<fp4::kMx, __nv_bfloat16>(a, b, out, K, sm_count, status_word, stream)
+                               : pair_product<fp4::kMx, __half>(a, b, out, K, sm_count, status_word, stream);
 }
 
 }  // namespace lbl

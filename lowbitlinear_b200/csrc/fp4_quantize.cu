@@ -25,8 +25,9 @@ template <typename T, int kFormat>
 __global__ void __launch_bounds__(kThreads)
     fp4_quantize_kernel(const T* __restrict__ x, int64_t row_stride, const float* __restrict__ factor,
                         uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int rows, int cols, int pitch,
-                        int tiles, int access) {
-  pdl_allow_next_kernel();
+                        int tiles, int access, bool early_successor) {
+  pdl_wait_for_previous_kernel();
+  if (early_successor) pdl_allow_next_kernel();
   const int lane = threadIdx.x & 31;
   const int row = blockIdx.y * blockDim.y + threadIdx.y;  // of this launch: fewer than 65536
   const int unit = blockIdx.x * blockDim.x + threadIdx.x;  // blockDim.x is a multiple of 32: a warp has one row
@@ -102,6 +103,7 @@ __global__ void __launch_bounds__(kThreads)
     fp4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                           const float* __restrict__ factor, T* __restrict__ out, int rows, int cols, int pitch,
                           int tiles, int access) {
+  pdl_wait_for_previous_kernel();
   const int lane = threadIdx.x & 31;
   const int row = blockIdx.y * blockDim.y + threadIdx.y;  // of this launch: fewer than 65536
   const int unit = blockIdx.x * blockDim.x + threadIdx.x;  // blockDim.x is a multiple of 32: a warp has one row
@@ -182,9 +184,23 @@ dim3 block_for(int64_t units) {
 
 constexpr int64_t kRowsPerLaunch = 65535 / 128 * 128;  // limit of the grid's y extent, in whole scale tiles
 
+template <typename... Parameters, typename... Arguments>
+cudaError_t launch(void (*kernel)(Parameters...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                   Arguments... arguments) {
+  cudaLaunchAttribute attr = fp4::programmatic_launch();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, Parameters(arguments)...);
+}
+
 template <typename T, int kFormat>
 cudaError_t quantize(const void* x, int64_t row_stride, const float* factor, uint8_t* codes, uint8_t* scales,
-                     int64_t rows, int64_t cols, cudaStream_t stream) {
+                     int64_t rows, int64_t cols, bool early_successor, cudaStream_t stream) {
   const int64_t tiles = fp4::scale_tiles(cols, kFormat);
   const int64_t units = tiles * fp4::Format<kFormat>::kTileCols / 16;
   const dim3 block = block_for(units);
@@ -197,11 +213,10 @@ cudaError_t quantize(const void* x, int64_t row_stride, const float* factor, uin
     const int64_t here = rows - r0 < kRowsPerLaunch ? rows - r0 : kRowsPerLaunch;
     const int64_t here_padded = (here + 127) / 128 * 128;
     const dim3 grid(static_cast<unsigned>(blocks_x), static_cast<unsigned>((here_padded + block.y - 1) / block.y));
-    fp4_quantize_kernel<T, kFormat><<<grid, block, smem, stream>>>(
-        static_cast<const T*>(x) + r0 * row_stride, row_stride, factor, codes + r0 * fp4::code_pitch(cols),
+    const cudaError_t err = launch(
+        fp4_quantize_kernel<T, kFormat>, grid, block, smem, stream, static_cast<const T*>(x) + r0 * row_stride, row_stride, factor, codes + r0 * fp4::code_pitch(cols),
         scales + r0 / 128 * tiles * 512, static_cast<int>(here), static_cast<int>(cols),
-        static_cast<int>(fp4::code_pitch(cols)), static_cast<int>(tiles), access);
-    const cudaError_t err = cudaGetLastError();
+        static_cast<int>(fp4::code_pitch(cols)), static_cast<int>(tiles), access, early_successor);
     if (err != cudaSuccess) return err;
   }
   return cudaSuccess;
@@ -220,11 +235,10 @@ cudaError_t dequantize(const uint8_t* codes, const uint8_t* scales, const float*
   for (int64_t r0 = 0; r0 < rows; r0 += kRowsPerLaunch) {
     const int64_t here = rows - r0 < kRowsPerLaunch ? rows - r0 : kRowsPerLaunch;
     const dim3 grid(static_cast<unsigned>(blocks_x), static_cast<unsigned>((here + block.y - 1) / block.y));
-    fp4_dequantize_kernel<T, kFormat><<<grid, block, smem, stream>>>(
-        codes + r0 * fp4::code_pitch(cols), scales + r0 / 128 * tiles * 512, factor, static_cast<T*>(out) + r0 * cols,
+    const cudaError_t err = launch(
+        fp4_dequantize_kernel<T, kFormat>, grid, block, smem, stream, codes + r0 * fp4::code_pitch(cols), scales + r0 / 128 * tiles * 512, factor, static_cast<T*>(out) + r0 * cols,
         static_cast<int>(here), static_cast<int>(cols), static_cast<int>(fp4::code_pitch(cols)), static_cast<int>(tiles),
         access);
-    const cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess) return err;
   }
   return cudaSuccess;
@@ -233,18 +247,19 @@ cudaError_t dequantize(const uint8_t* codes, const uint8_t* scales, const float*
 }  // namespace
 
 cudaError_t launch_fp4_quantize(const void* x, int x_type, int64_t row_stride, int format, const float* factor,
-                                uint8_t* codes, uint8_t* scales, int64_t rows, int64_t cols, cudaStream_t stream) {
+                                uint8_t* codes, uint8_t* scales, int64_t rows, int64_t cols, bool early_successor,
+                                cudaStream_t stream) {
   const bool nv = format == fp4::kNv;
   switch (x_type) {
     case kTypeF16:
-      return nv ? quantize<__half, fp4::kNv>(x, row_stride, factor, codes, scales, rows, cols, stream)
-                : quantize<__half, fp4::kMx>(x, row_stride, factor, codes, scales, rows, cols, stream);
+      return nv ? quantize<__half, fp4::kNv>(x, row_stride, factor, codes, scales, rows, cols, early_successor, stream)
+                : quantize<__half, fp4::kMx>(x, row_stride, factor, codes, scales, rows, cols, early_successor, stream);
     case kTypeBf16:
-      return nv ? quantize<__nv_bfloat16, fp4::kNv>(x, row_stride, factor, codes, scales, rows, cols, stream)
-                : quantize<__nv_bfloat16, fp4::kMx>(x, row_stride, factor, codes, scales, rows, cols, stream);
+      return nv ? quantize<__nv_bfloat16, fp4::kNv>(x, row_stride, factor, codes, scales, rows, cols, early_successor, stream)
+                : quantize<__nv_bfloat16, fp4::kMx>(x, row_stride, factor, codes, scales, rows, cols, early_successor, stream);
     case kTypeF32:
-      return nv ? quantize<float, fp4::kNv>(x, row_stride, factor, codes, scales, rows, cols, stream)
-                : quantize<float, fp4::kMx>(x, row_stride, factor, codes, scales, rows, cols, stream);
+      return nv ? quantize<float, fp4::kNv>(x, row_stride, factor, codes, scales, rows, cols, early_successor, stream)
+                : quantize<float, fp4::kMx>(x, row_stride, factor, codes, scales, rows, cols, early_successor, stream);
   }
   return cudaErrorInvalidValue;
 }

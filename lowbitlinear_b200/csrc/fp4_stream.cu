@@ -40,6 +40,7 @@ struct StreamParams {
   int split;        // CTAs of a cluster, a power of two
   int split_shift;  // its logarithm
   int x_access;     // how rows of x may be read
+  int early_weight;  // fetch the weight before the kernel in front is complete
   int receive_offset;  // where partial sums arrive in shared memory; 0: over the ring
   int* status;
 };
@@ -174,8 +175,8 @@ __global__ void __launch_bounds__(StreamTile<kFormat, kQ, kFused>::kThreads, 2)
   };
   const int ahead = min(p.stages, stages_here);
 
-  // The weight's first stages are on their way before anything else is set up.  The activations may come from
-  // the kernel in front of this one, the weight does not (a call's own quantiser is that kernel).
+  // The weight's first stages are on their way before anything else is set up.  The activations may come from the
+  // kernel in front of this one; the weight does not when that is the call's own quantiser or the caller says so.
   if (warp == 0) {
     if (elect_one()) {
       for (int s = 0; s < p.stages; ++s) {
@@ -185,6 +186,7 @@ __global__ void __launch_bounds__(StreamTile<kFormat, kQ, kFused>::kThreads, 2)
       mbar_init(&bars.done, 1);
       bars.abort_flag = 0;
       mbar_init_fence();
+      if (!p.early_weight) pdl_wait_for_previous_kernel();
       for (int i = 0; i < ahead; ++i) load_p(i);
       if constexpr (!kFused) {
         pdl_wait_for_previous_kernel();
@@ -343,7 +345,7 @@ int stages_of(int64_t K) { return static_cast<int>((fp4::padded_cols(K) + kStage
 
 template <int kFormat, int kQ, bool kFused, typename T>
 cudaError_t launch(const Fp4Operand& w, const Fp4Operand& x, const void* raw, int64_t raw_stride, void* out, int64_t K,
-                   int sm_count, int* status, bool pdl, cudaStream_t stream) {
+                   int sm_count, int* status, bool early_weight, cudaStream_t stream) {
   using Tile = StreamTile<kFormat, kQ, kFused>;
   const int64_t pitch = fp4::code_pitch(K);
   CUtensorMap map_p, map_q;
@@ -419,11 +421,7 @@ cudaError_t launch(const Fp4Operand& w, const Fp4Operand& x, const void* raw, in
     attr[attrs].val.clusterDim.z = 1;
     ++attrs;
   }
-  if (pdl) {
-    attr[attrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[attrs].val.programmaticStreamSerializationAllowed = 1;
-    ++attrs;
-  }
+  attr[attrs++] = fp4::programmatic_launch();
   cfg.attrs = attr;
   cfg.numAttrs = attrs;
   return cudaLaunchKernelEx(&cfg, kernel, map_p, map_q, params);
@@ -433,21 +431,21 @@ cudaError_t launch(const Fp4Operand& w, const Fp4Operand& x, const void* raw, in
 
 template <int kFormat, typename T>
 static cudaError_t stream_product(const Fp4Operand& a, const Fp4Operand& b, void* out, int64_t K, int sm_count,
-                                  int* status, bool pdl, cudaStream_t stream) {
-  if (a.rows <= 16) return launch<kFormat, 16, false, T>(b, a, nullptr, 0, out, K, sm_count, status, pdl, stream);
-  if (a.rows <= 32) return launch<kFormat, 32, false, T>(b, a, nullptr, 0, out, K, sm_count, status, pdl, stream);
-  if (a.rows <= 64) return launch<kFormat, 64, false, T>(b, a, nullptr, 0, out, K, sm_count, status, pdl, stream);
-  return launch<kFormat, 128, false, T>(b, a, nullptr, 0, out, K, sm_count, status, pdl, stream);
+                                  int* status, bool early_weight, cudaStream_t stream) {
+  if (a.rows <= 16) return launch<kFormat, 16, false, T>(b, a, nullptr, 0, out, K, sm_count, status, early_weight, stream);
+  if (a.rows <= 32) return launch<kFormat, 32, false, T>(b, a, nullptr, 0, out, K, sm_count, status, early_weight, stream);
+  if (a.rows <= 64) return launch<kFormat, 64, false, T>(b, a, nullptr, 0, out, K, sm_count, status, early_weight, stream);
+  return launch<kFormat, 128, false, T>(b, a, nullptr, 0, out, K, sm_count, status, early_weight, stream);
 }
 
 cudaError_t launch_fp4_stream(const Fp4Operand& a, const Fp4Operand& b, int format, void* out, int out_type, int64_t K,
-                              int sm_count, int* status_word, bool pdl, cudaStream_t stream) {
+                              int sm_count, int* status_word, bool early_weight, cudaStream_t stream) {
   if (format == fp4::kNv) {
-    return out_type == kTypeBf16 ? stream_product<fp4::kNv, __nv_bfloat16>(a, b, out, K, sm_count, status_word, pdl, stream)
-                                 : stream_product<fp4::kNv, __half>(a, b, out, K, sm_count, status_word, pdl, stream);
+    return out_type == kTypeBf16 ? stream_product<fp4::kNv, __nv_bfloat16>(a, b, out, K, sm_count, status_word, early_weight, stream)
+                                 : stream_product<fp4::kNv, __half>(a, b, out, K, sm_count, status_word, early_weight, stream);
   }
-  return out_type == kTypeBf16 ? stream_product<fp4::kMx, __nv_bfloat16>(a, b, out, K, sm_count, status_word, pdl, stream)
-                               : stream_product<fp4::kMx, __half>(a, b, out, K, sm_count, status_word, pdl, stream);
+  return out_type == kTypeBf16 ? stream_product<fp4::kMx, __nv_bfloat16>(a, b, out, K, sm_count, status_word, early_weight, stream)
+                               : stream_product<fp4::kMx, __half>(a, b, out, K, sm_count, status_word, early_weight, stream);
 }
 
 // Every CTA rounds its slice of the activations itself: worth a launch while that is a step or two.
@@ -460,16 +458,16 @@ bool fp4_fused_supports(int64_t M, int64_t N, int64_t K, int sm_count) {
 
 cudaError_t launch_fp4_fused_linear(const void* x, int x_type, int64_t x_stride, int64_t M, const float* x_factor,
                                     const Fp4Operand& w, int format, void* out, int64_t K, int sm_count,
-                                    int* status_word, bool pdl, cudaStream_t stream) {
+                                    int* status_word, bool early_weight, cudaStream_t stream) {
   const Fp4Operand a = {nullptr, nullptr, x_factor, M};
   if (format == fp4::kNv) {
     return x_type == kTypeBf16
-               ? launch<fp4::kNv, kFusedRows, true, __nv_bfloat16>(w, a, x, x_stride, out, K, sm_count, status_word, pdl, stream)
-               : launch<fp4::kNv, kFusedRows, true, __half>(w, a, x, x_stride, out, K, sm_count, status_word, pdl, stream);
+               ? launch<fp4::kNv, kFusedRows, true, __nv_bfloat16>(w, a, x, x_stride, out, K, sm_count, status_word, early_weight, stream)
+               : launch<fp4::kNv, kFusedRows, true, __half>(w, a, x, x_stride, out, K, sm_count, status_word, early_weight, stream);
   }
   return x_type == kTypeBf16
-             ? launch<fp4::kMx, kFusedRows, true, __nv_bfloat16>(w, a, x, x_stride, out, K, sm_count, status_word, pdl, stream)
-             : launch<fp4::kMx, kFusedRows, true, __half>(w, a, x, x_stride, out, K, sm_count, status_word, pdl, stream);
+             ? launch<fp4::kMx, kFusedRows, true, __nv_bfloat16>(w, a, x, x_stride, out, K, sm_count, status_word, early_weight, stream)
+             : launch<fp4::kMx, kFusedRows, true, __half>(w, a, x, x_stride, out, K, sm_count, status_word, early_weight, stream);
 }
 
 }  // namespace lbl

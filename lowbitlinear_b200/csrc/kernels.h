@@ -175,8 +175,10 @@ constexpr int kTypeBf16 = 1;
 constexpr int kTypeF32 = 2;
 // x [rows, cols] with `row_stride` elements between rows -> codes [rows, 16 ceil(cols / 32)], tiled scales
 // (padding rows and blocks written as zero).  factor: FP32 tensor factor of NVFP4 on the device, null = 1.
+// `early_successor`: the next kernel of the stream may start beside this one (it waits before it reads the result).
 cudaError_t launch_fp4_quantize(const void* x, int x_type, int64_t row_stride, int format, const float* factor,
-                                uint8_t* codes, uint8_t* scales, int64_t rows, int64_t cols, cudaStream_t stream);
+                                uint8_t* codes, uint8_t* scales, int64_t rows, int64_t cols, bool early_successor,
+                                cudaStream_t stream);
 cudaError_t launch_fp4_dequantize(const uint8_t* codes, const uint8_t* scales, int format, const float* factor,
                                   void* out, int out_type, int64_t rows, int64_t cols, cudaStream_t stream);
 struct Fp4Operand {
@@ -186,17 +188,17 @@ struct Fp4Operand {
   int64_t rows;
 };
 // out [a.rows, b.rows] = a . b^T, FP16 or BF16; K >= 1, rows >= 1, codes and scales 16-byte aligned.
-// `pdl`: programmatic dependent launch; b (the weight) must not be written by the kernel in front.
+// `early_weight`: b is fetched before the kernel in front is complete, which must not write it.
 // Few rows of a (fp4_stream.cu): b is streamed once, K is cut into slices that meet in a cluster.
 cudaError_t launch_fp4_stream(const Fp4Operand& a, const Fp4Operand& b, int format, void* out, int out_type, int64_t K,
-                              int sm_count, int* status_word, bool pdl, cudaStream_t stream);
+                              int sm_count, int* status_word, bool early_weight, cudaStream_t stream);
 // The same with a given as 16-bit activations x [M, K], quantised in the kernel; out has their type.
 bool fp4_fused_supports(int64_t M, int64_t N, int64_t K, int sm_count);
 cudaError_t launch_fp4_fused_linear(const void* x, int x_type, int64_t x_stride, int64_t M, const float* x_factor,
                                     const Fp4Operand& w, int format, void* out, int64_t K, int sm_count,
-                                    int* status_word, bool pdl, cudaStream_t stream);
+                                    int* status_word, bool early_weight, cudaStream_t stream);
 // Many rows of both (fp4_pair.cu): persistent 256 x 256 tiles on pairs of CTAs.
 cudaError_t launch_fp4_pair(const Fp4Operand& a, const Fp4Operand& b, int format, void* out, int out_type, int64_t K,
-                            int sm_count, int* status_word, bool pdl, cudaStream_t stream);
+                            int sm_count, int* status_word, cudaStream_t stream);
 
 }  // namespace lbl
