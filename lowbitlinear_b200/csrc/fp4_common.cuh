@@ -50,8 +50,8 @@ __device__ __forceinline__ float e4m3_to_float(uint32_t byte) {
   return static_cast<float>(v);
 }
 
-// What one block needs to round its values.  mul + mul_low is the reciprocal of the step, mul rounded down (MXFP4: mul
-// alone, exact).
+// What one block needs to round its values.  mul + mul_low is the reciprocal of the step to more than 40 bits, mul a
+// little below it (MXFP4: mul alone, exact).
 struct BlockStep {
   uint32_t byte;  // scale as stored
   float step, mul, mul_low;
@@ -110,7 +110,8 @@ __device__ __forceinline__ BlockStep nv_step(uint32_t amax_bits, const TensorFac
   b.byte = bad ? 0x7Fu : byte;
   b.step = e4m3_to_float(byte) * f.g;
   const bool none = bad || byte == 0;  // a step of zero: every code is zero
-  b.mul = none ? 0.0f : __frcp_rd(b.step);
+  // The quotient is off by two units in the last place at most; 2^-21 below it lies under the reciprocal for certain.
+  b.mul = none ? 0.0f : __fdividef(1.0f - 0x1p-21f, b.step);
   b.mul_low = none ? 0.0f : fmaf(-b.mul, b.step, 1.0f) * b.mul;
   b.short_step = f.power_of_two;
   b.limit = byte >= 0x7Eu ? 8.0f * b.step : __uint_as_float(0x7F800000u);
@@ -131,28 +132,36 @@ __device__ __forceinline__ uint32_t eight_codes(const float (&q)[8]) {
   return out;
 }
 
-// Codes of eight neighbouring values.  kHalfInput: they were FP16 or BF16 numbers.
-template <int kFormat, bool kHalfInput>
-__device__ __forceinline__ uint32_t round_eight(const float (&x)[8], const BlockStep& b) {
-  float q[8];
-  if constexpr (kFormat == kMx) {
+// Codes of sixteen neighbouring values (Sixteen<T> below).
+template <int kFormat, typename Values>
+__device__ __forceinline__ uint2 round_sixteen(const Values& v, const BlockStep& b) {
+  uint32_t codes[2];
+  float x[8], q[8];
+  if (kFormat == kMx || (Values::kHalf && b.short_step)) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = x[i] * b.mul;
-  } else if (kHalfInput && b.short_step) {
-    // The quotient to 47 bits, rounded once.  A number of at most eleven bits is either on a border (at most seven
-    // bits: three of the code's border, four of the step), and then comes out as the border itself, or at least 2^-11
-    // of it away.  Both products have the sign of x, zeros included.
+    for (int h = 0; h < 2; ++h) {
+      v.eight(h, x);
+      // NVFP4: the quotient to 40 bits, rounded once.  A number of at most eleven bits is either on a border (at most
+      // seven bits: three of the code's border, four of the step), and then comes out as the border itself, or at
+      // least 2^-11 of it away.  Both products have the sign of x, zeros included.
 #pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = fmaf(x[i], b.mul, x[i] * b.mul_low);
+      for (int i = 0; i < 8; ++i) q[i] = kFormat == kMx ? x[i] * b.mul : fmaf(x[i], b.mul, x[i] * b.mul_low);
+      codes[h] = eight_codes(q);
+    }
   } else {
-    // Only a saturated scale (8 steps < amax) makes the bound finite.  The sign of a zero is kept.
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      q[i] = copysignf(sided_quotient(fminf(fabsf(x[i]), b.limit), b.step, b.mul), x[i]);
+    for (int h = 0; h < 2; ++h) {
+      v.eight(h, x);
+      // Only a saturated scale (8 steps < amax) makes the bound finite.  The sign of a zero is kept.
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        q[i] = copysignf(sided_quotient(fminf(fabsf(x[i]), b.limit), b.step, b.mul), x[i]);
+      }
+      codes[h] = eight_codes(q);
     }
   }
-  const uint32_t codes = eight_codes(q);
-  return b.byte == Format<kFormat>::kNanScale ? 0u : codes;
+  const bool bad = b.byte == Format<kFormat>::kNanScale;
+  return make_uint2(bad ? 0u : codes[0], bad ? 0u : codes[1]);
 }
 
 // Eight codes as four pairs of FP16 numbers in column order (exact).
@@ -217,6 +226,7 @@ template <typename T>
 struct Sixteen;
 template <>
 struct Sixteen<float> {
+  static constexpr bool kHalf = false;
   float v[16];
   __device__ __forceinline__ void load_vector(const float* p, int access) {
     if (access == kRows32) {
@@ -264,7 +274,23 @@ __device__ __forceinline__ float2 pair_to_float<__nv_bfloat16>(uint32_t bits) {
 }
 
 template <typename T>
+__device__ __forceinline__ uint32_t max_magnitude(uint32_t a, uint32_t b);
+template <>
+__device__ __forceinline__ uint32_t max_magnitude<__half>(uint32_t a, uint32_t b) {
+  uint32_t m;
+  asm("max.NaN.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
+  return m;
+}
+template <>
+__device__ __forceinline__ uint32_t max_magnitude<__nv_bfloat16>(uint32_t a, uint32_t b) {
+  uint32_t m;
+  asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
+  return m;
+}
+
+template <typename T>
 struct SixteenHalves {
+  static constexpr bool kHalf = true;
   uint32_t w[8];
   __device__ __forceinline__ void load_vector(const T* p, int access) {
     if (access == kRows32) {
@@ -284,10 +310,12 @@ struct SixteenHalves {
       w[i] = lo | (hi << 16);
     }
   }
+  // Magnitudes two at a time; the sign of the running maximum is noise until the end, NaN stays.
   __device__ __forceinline__ uint32_t amax_bits() const {
-    uint32_t m = 0;
+    uint32_t m = w[0];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) asm("max.u16x2 %0, %0, %1;" : "+r"(m) : "r"(w[i] & 0x7FFF7FFFu));
+    for (int i = 1; i < 8; ++i) m = max_magnitude<T>(m, w[i]);
+    m &= 0x7FFF7FFFu;
     const uint32_t top = max(m & 0xFFFFu, m >> 16);
     return __float_as_uint(pair_to_float<T>(top).x);
   }

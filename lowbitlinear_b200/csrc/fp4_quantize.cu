@@ -62,12 +62,7 @@ __global__ void __launch_bounds__(kThreads)
   } else {
     step = fp4::nv_step(amax, fp4::tensor_factor(factor));
   }
-  float part[8];
-  uint2 out;
-  v.eight(0, part);
-  out.x = fp4::round_eight<kFormat, sizeof(T) == 2>(part, step);
-  v.eight(1, part);
-  out.y = fp4::round_eight<kFormat, sizeof(T) == 2>(part, step);
+  const uint2 out = fp4::round_sixteen<kFormat>(v, step);
   const bool stored = row < rows && unit * 8 < pitch;
   if (stored) *reinterpret_cast<uint2*>(codes + static_cast<int64_t>(row) * pitch + unit * 8) = out;
 

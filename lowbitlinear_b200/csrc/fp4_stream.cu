@@ -104,12 +104,7 @@ __device__ __forceinline__ void quantise_slice(const StreamParams& p, int k_begi
     } else {
       step = fp4::nv_step(amax, factor);
     }
-    float part[8];
-    uint2 out;
-    v.eight(0, part);
-    out.x = fp4::round_eight<kFormat, true>(part, step);
-    v.eight(1, part);
-    out.y = fp4::round_eight<kFormat, true>(part, step);
+    const uint2 out = fp4::round_sixteen<kFormat>(v, step);
     if (have) {
       const uint32_t chunk = unit >> 1;
       uint8_t* dst = codes + stage * Tile::kBytesQ + (row >> 3) * 1024 + (row & 7) * 128 +
