@@ -271,7 +271,8 @@ int lbl_w4a16_dequantize(const int32_t* packed_w, const float* scales, const int
 /* ---- Microscaled 4-bit floating point --------------------------------------------------------
  * Formats with E2M1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign) and one scale per block of columns:
  *   LBL_FP4_MX  blocks of 32, E8M0 scale byte: step = 2^(byte - 127)
- *   LBL_FP4_NV  blocks of 16, E4M3 scale byte and one FP32 factor g per tensor: step = scale * g
+ *   LBL_FP4_NV  blocks of 16, E4M3 scale byte (bit 7 clear) and one FP32 factor g per tensor:
+ *               step = scale * g
  * An operand [R, K] is stored as
  *   codes   uint8 [R, 16 * ceil(K / 32)], two codes to a byte, low nibble first, zero past column K
  *   scales  uint8 [ceil(R / 128), ceil(blocks / 4), 32, 4, 4] (blocks: of the columns padded to 32): the
@@ -279,7 +280,8 @@ int lbl_w4a16_dequantize(const int32_t* packed_w, const float* scales, const int
  * Factors are pointers to one float on the device, null meaning 1; they belong to LBL_FP4_NV only
  * (LBL_ERR_INVALID otherwise).  Codes and scales have to be 16-byte aligned, activations and outputs
  * aligned to their type.  Rows and columns up to 2^30.  No call allocates, synchronises or retains
- * anything; all can be captured. */
+ * anything; all can be captured.  Of the flags LBL_FLAG_PDL counts: b (the weight) is fetched before the
+ * kernel in front of the call is complete, which must not write it. */
 #define LBL_FP4_MX 0
 #define LBL_FP4_NV 1
 #define LBL_TYPE_F16 0

@@ -541,6 +541,7 @@ def _pointer(tensor):
 
 
 def _contiguous_rows(x):
+    x = x.resolve_neg()
     return x if x.stride(1) == 1 and x.stride(0) >= 0 else x.contiguous()
 
 

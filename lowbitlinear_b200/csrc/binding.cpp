@@ -28,11 +28,11 @@ struct EntryPoints {
 
 constexpr int64_t kMostColumns = int64_t{1} << 30;
 
-// A plain tensor on a GPU (no subclass, which may have its own ideas), or null.
+// A plain tensor on a GPU (no subclass, which may have its own ideas, and no view that negates), or null.
 const at::Tensor* cuda_tensor(PyObject* object) {
   if (!THPVariable_CheckExact(object)) return nullptr;
   const at::Tensor& t = THPVariable_Unpack(object);
-  return t.is_cuda() && t.layout() == at::kStrided ? &t : nullptr;
+  return t.is_cuda() && t.layout() == at::kStrided && !t.is_neg() ? &t : nullptr;
 }
 
 int format_code(PyObject* object) {

@@ -17,7 +17,8 @@ and zero codes, so that it reads back as NaN.
 Storage: ``codes`` uint8 ``[R, 16 ceil(K / 32)]``, two codes to a byte, low nibble first, zero past
 column K; ``scales`` uint8 ``[ceil(R / 128), ceil(blocks / 4), 32, 4, 4]``: the byte of row ``r`` and
 block ``j`` lies at ``[r // 128, j // 4, r % 32, r % 128 // 32, j % 4]``, the order in which the tensor
-cores take it, and bytes without a row or block are zero (``blocks`` counts the padded columns).
+cores take it, and bytes without a row or block are zero (``blocks`` counts the padded columns).  The tensor cores
+read an E4M3 scale without its sign, so bit 7 of an nvfp4 scale is clear.
 ``tile_scales`` and ``untile_scales`` convert from and to plain ``[R, blocks]`` rows, as checkpoints
 store them.
 

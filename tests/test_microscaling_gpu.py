@@ -121,9 +121,11 @@ def test_product_matches_64_bits(cuda_ops, fmt, m, n, k):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
-@pytest.mark.parametrize("m,n,k", [(1030, 2100, 320), (1537, 2048, 33), (257, 9601, 1500), (4097, 1000, 100), (2000, 4096, 2048)])
+@pytest.mark.parametrize("m,n,k", [(1030, 2100, 320), (1537, 2048, 33), (257, 9601, 1500), (4097, 1000, 100), (2000, 4096, 2048),
+                                   (200, 6150, 1100), (513, 2304, 4096)])
 def test_large_products_match_64_bits(cuda_ops, fmt, m, n, k):
-    """Persistent tiles: several per CTA pair, ragged edges, rows past the last one in half of a pair."""
+    """Persistent tiles: several per CTA pair, ragged edges, rows past the last one in half of a pair; the last two
+    have so few tiles that two pairs share each."""
     test_product_matches_64_bits(cuda_ops, fmt, m, n, k)
 
 
