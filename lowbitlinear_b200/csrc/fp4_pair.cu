@@ -220,7 +220,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == 0) {
     const uint32_t full = map_to_cta(smem_addr(&bars.full[0]), leader);
-    int i = 0;  // stages since the start
+    RingPosition at;
+    at.parity = 1;  // the first round finds every stage free
     for (int t = first_tile; t < tiles; t += tile_step) {
       int tile_a, tile_b;
       tile_of(p, t, &tile_a, &tile_b);
@@ -228,10 +229,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int row_a = tile_a * kRowsPair + static_cast<int>(rank) * kRowsCta;
       const int row_b = tile_b * kRowsPair + static_cast<int>(rank) * kRowsCta;
       bool ok = true;
-      for (int kb = kb_begin; kb < kb_end; ++kb, ++i) {
-        const int s = i % Tile::kStages;
-        const int round = i / Tile::kStages;
-        ok = round == 0 || warp_wait(&bars.empty[s], (round - 1) & 1, abort_flag, p.status, kStatusPairWait + 1);
+      for (int kb = kb_begin; kb < kb_end; ++kb, at.next(Tile::kStages)) {
+        const int s = at.slot;
+        ok = warp_wait(&bars.empty[s], at.parity, abort_flag, p.status, kStatusPairWait + 1);
         if (!ok) break;
         if (elect_one()) {
           if (rank == 0) mbar_arrive_expect_tx(&bars.full[s], 2 * Tile::kStageBytes);
@@ -247,7 +247,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == 1) {
     if (rank == 0) {
-      int i = 0, n = 0;
+      const uint32_t a_addr = smem_addr(smem_a), b_addr = smem_addr(smem_b);
+      const uint32_t sa_addr = smem_addr(smem_sa), sb_addr = smem_addr(smem_sb);
+      RingPosition at;
+      int n = 0;
       for (int t = first_tile; t < tiles; t += tile_step, ++n) {
         // Tile n may use its accumulator once the epilogue has read the shared columns of tile n - 1 (and with
         // them, in program order, all of tile n - 2).
@@ -255,16 +258,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         tc_fence_after_sync();
         const uint32_t acc = tmem + (n & 1) * kSecondAccumulator;
-        for (int kb = kb_begin; kb < kb_end; ++kb, ++i) {
-          const int s = i % Tile::kStages;
-          ok = warp_wait(&bars.full[s], (i / Tile::kStages) & 1, abort_flag, p.status, kStatusPairWait + 3);
+        for (int kb = kb_begin; kb < kb_end; ++kb, at.next(Tile::kStages)) {
+          const int s = at.slot;
+          ok = warp_wait(&bars.full[s], at.parity, abort_flag, p.status, kStatusPairWait + 3);
           if (!ok) break;
           tc_fence_after_sync();
           if (elect_one()) {
             issue_stage<kFormat, 2, kRowsPair, kRowsPair>(
-                acc, tmem + kScaleColumn, smem_addr(smem_a + s * Tile::kBytesCodes),
-                smem_addr(smem_b + s * Tile::kBytesCodes), smem_addr(smem_sa + s * Tile::kBytesScaleA),
-                smem_addr(smem_sb + s * Tile::kBytesScaleB), p.cols_padded - kb * kStageCols, kb == kb_begin);
+                acc, tmem + kScaleColumn, a_addr + s * Tile::kBytesCodes, b_addr + s * Tile::kBytesCodes,
+                sa_addr + s * Tile::kBytesScaleA, sb_addr + s * Tile::kBytesScaleB, p.cols_padded - kb * kStageCols,
+                kb != kb_begin);
             mma_commit_pair(&bars.empty[s], leader);
             if (kb == kb_end - 1) mma_commit_pair(&bars.acc_full, leader);
           }

@@ -145,9 +145,8 @@ __global__ void __launch_bounds__(StreamTile<kFormat, kQ, kFused>::kThreads, 2)
   uint8_t* smem_sq = smem_sp + p.stages * Tile::kBytesScaleP;
 
   const int tile_step = Tile::kTiles;
-  auto load_p = [&](int i) {
+  auto load_p = [&](int i, int s) {
     const int kb = k_begin + i;
-    const int s = i % p.stages;
     const uint32_t bytes = min(tile_step, p.scale_tiles - kb * tile_step) * 512;
     int blocks_q = 0;
     if (!kFused) {
@@ -158,9 +157,8 @@ __global__ void __launch_bounds__(StreamTile<kFormat, kQ, kFused>::kThreads, 2)
     bulk_load(smem_sp + s * Tile::kBytesScaleP,
               p.sf_p + (static_cast<int64_t>(p0 / 128) * p.scale_tiles + kb * tile_step) * 512, bytes, &bars.full[s]);
   };
-  auto load_q = [&](int i) {
+  auto load_q = [&](int i, int s) {
     const int kb = k_begin + i;
-    const int s = i % p.stages;
     const uint32_t bytes = min(tile_step, p.scale_tiles - kb * tile_step) * 512;
     tma_load_2d(smem_q + s * Tile::kBytesQ, &map_q, kb * kRowBytes, q0, &bars.full[s]);
     for (int b = 0; b < Tile::kQBlocks && b * 128 < used; ++b) {
@@ -182,10 +180,10 @@ __global__ void __launch_bounds__(StreamTile<kFormat, kQ, kFused>::kThreads, 2)
       bars.abort_flag = 0;
       mbar_init_fence();
       if (!p.early_weight) pdl_wait_for_previous_kernel();
-      for (int i = 0; i < ahead; ++i) load_p(i);
+      for (int i = 0; i < ahead; ++i) load_p(i, i);
       if constexpr (!kFused) {
         pdl_wait_for_previous_kernel();
-        for (int i = 0; i < ahead; ++i) load_q(i);
+        for (int i = 0; i < ahead; ++i) load_q(i, i);
       }
     }
     __syncwarp();
@@ -209,25 +207,28 @@ __global__ void __launch_bounds__(StreamTile<kFormat, kQ, kFused>::kThreads, 2)
   pdl_allow_next_kernel();
 
   if (warp == 0) {
-    for (int i = ahead; i < stages_here; ++i) {
-      if (!warp_wait(&bars.empty[i % p.stages], (i / p.stages - 1) & 1, abort_flag, p.status, kStatusStreamWait + 1)) break;
+    RingPosition at;
+    for (int i = ahead; i < stages_here; ++i, at.next(p.stages)) {
+      if (!warp_wait(&bars.empty[at.slot], at.parity, abort_flag, p.status, kStatusStreamWait + 1)) break;
       if (elect_one()) {
-        load_p(i);
-        if constexpr (!kFused) load_q(i);
+        load_p(i, at.slot);
+        if constexpr (!kFused) load_q(i, at.slot);
       }
       __syncwarp();
     }
   } else if (warp == 1) {
-    for (int i = 0; i < stages_here; ++i) {
-      const int s = i % p.stages;
-      if (!warp_wait(&bars.full[s], (i / p.stages) & 1, abort_flag, p.status, kStatusStreamWait + 2)) break;
+    const uint32_t p_addr = smem_addr(smem_p), q_addr = smem_addr(smem_q);
+    const uint32_t sp_addr = smem_addr(smem_sp), sq_addr = smem_addr(smem_sq);
+    RingPosition at;
+    for (int i = 0; i < stages_here; ++i, at.next(p.stages)) {
+      const int s = at.slot;
+      if (!warp_wait(&bars.full[s], at.parity, abort_flag, p.status, kStatusStreamWait + 2)) break;
       tc_fence_after_sync();
       const int sq = kFused ? i : s;
       if (elect_one()) {
-        issue_stage<kFormat, 1, kP, kQ>(tmem, tmem + kQ, smem_addr(smem_p + s * Tile::kBytesP),
-                                        smem_addr(smem_q + sq * Tile::kBytesQ), smem_addr(smem_sp + s * Tile::kBytesScaleP),
-                                        smem_addr(smem_sq + sq * Tile::kBytesScaleQ),
-                                        p.cols_padded - (k_begin + i) * kStageCols, i == 0);
+        issue_stage<kFormat, 1, kP, kQ>(tmem, tmem + kQ, p_addr + s * Tile::kBytesP, q_addr + sq * Tile::kBytesQ,
+                                        sp_addr + s * Tile::kBytesScaleP, sq_addr + sq * Tile::kBytesScaleQ,
+                                        p.cols_padded - (k_begin + i) * kStageCols, i != 0);
         mma_commit(&bars.empty[s]);
         if (i == stages_here - 1) mma_commit(&bars.done);
       }

@@ -75,11 +75,11 @@ __device__ __forceinline__ void mma_fp4(uint32_t d_tmem, uint64_t a_desc, uint64
 #undef LBL_FP4_MMA
 
 // Copies the scale tiles of one stage and issues its MMAs.  kRowsP / kRowsQ: rows of the instruction;
-// scales of P: one 128-row tile per CTA, of Q: kQBlocks tiles.  The last stage of K issues only the MMAs that
-// have columns, so no scale byte is used that was not loaded.
-template <int kFormat, int kCtas, int kRowsP, int kRowsQ>
+// scales of P: one 128-row tile per CTA, of Q: kQBlocks tiles.  The last stage of K (not kWhole) issues only the MMAs
+// that have columns, so no scale byte is used that was not loaded.
+template <int kFormat, int kCtas, int kRowsP, int kRowsQ, bool kWhole>
 __device__ __forceinline__ void issue_stage(uint32_t d_tmem, uint32_t sf_tmem, uint32_t p_addr, uint32_t q_addr,
-                                            uint32_t sf_p_addr, uint32_t sf_q_addr, int cols_left, bool first) {
+                                            uint32_t sf_p_addr, uint32_t sf_q_addr, int cols_left, uint32_t accumulate) {
   constexpr int kTileCols = fp4::Format<kFormat>::kTileCols;
   constexpr int kTiles = kStageCols / kTileCols;
   constexpr int kQBlocks = (kRowsQ + 127) / 128;
@@ -87,7 +87,7 @@ __device__ __forceinline__ void issue_stage(uint32_t d_tmem, uint32_t sf_tmem, u
   const uint32_t sf_q = sf_tmem + kTiles * 4;
 #pragma unroll
   for (int t = 0; t < kTiles; ++t) {
-    if (t * kTileCols < cols_left) {
+    if (kWhole || t * kTileCols < cols_left) {
       scales_to_tmem<kCtas>(sf_p + t * 4, sf_p_addr + t * 512);
 #pragma unroll
       for (int b = 0; b < kQBlocks; ++b) {
@@ -95,16 +95,27 @@ __device__ __forceinline__ void issue_stage(uint32_t d_tmem, uint32_t sf_tmem, u
       }
     }
   }
+  const uint64_t p_desc = smem_desc_k_major_sw128(p_addr);
+  const uint64_t q_desc = smem_desc_k_major_sw128(q_addr);
 #pragma unroll
   for (int j = 0; j < kStageCols / kMmaCols; ++j) {
-    if (j * kMmaCols < cols_left) {
-      // MXFP4: a scale tile serves two MMAs, bytes 0-1 and 2-3; NVFP4: one.
+    if (kWhole || j * kMmaCols < cols_left) {
+      // MXFP4: a scale tile serves two MMAs, bytes 0-1 and 2-3; NVFP4: one.  64 columns are 32 bytes: two units of the
+      // descriptors' addresses.
       const int t = kFormat == fp4::kMx ? j / 2 : j;
       const uint32_t id = kFormat == fp4::kMx ? (j & 1) * 2u : 0u;
-      mma_fp4<kFormat, kCtas>(d_tmem, smem_desc_k_major_sw128(p_addr + j * 32), smem_desc_k_major_sw128(q_addr + j * 32),
-                              fp4_instr_desc<kFormat>(kRowsP, kRowsQ, id), sf_p + t * 4, sf_q + t * 4 * kQBlocks,
-                              first && j == 0 ? 0u : 1u);
+      mma_fp4<kFormat, kCtas>(d_tmem, p_desc + 2 * j, q_desc + 2 * j, fp4_instr_desc<kFormat>(kRowsP, kRowsQ, id),
+                              sf_p + t * 4, sf_q + t * 4 * kQBlocks, j == 0 ? accumulate : 1u);
     }
+  }
+}
+template <int kFormat, int kCtas, int kRowsP, int kRowsQ>
+__device__ __forceinline__ void issue_stage(uint32_t d_tmem, uint32_t sf_tmem, uint32_t p_addr, uint32_t q_addr,
+                                            uint32_t sf_p_addr, uint32_t sf_q_addr, int cols_left, uint32_t accumulate) {
+  if (cols_left >= kStageCols) {
+    issue_stage<kFormat, kCtas, kRowsP, kRowsQ, true>(d_tmem, sf_tmem, p_addr, q_addr, sf_p_addr, sf_q_addr, cols_left, accumulate);
+  } else {
+    issue_stage<kFormat, kCtas, kRowsP, kRowsQ, false>(d_tmem, sf_tmem, p_addr, q_addr, sf_p_addr, sf_q_addr, cols_left, accumulate);
   }
 }
 
@@ -128,12 +139,27 @@ __device__ __forceinline__ bool mbar_spin_bounded(uint64_t* bar, uint32_t parity
   }
 }
 
-// The same for all lanes of a warp, with one verdict: false when anybody has given up.
+// The same for all lanes of a warp, with one verdict: false when anybody has given up.  A phase that is already
+// complete costs one poll and one vote: the loops that issue copies and MMAs have 500 cycles per stage, and every
+// instruction in front of them counts.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status_word,
                                           int status_code) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
   mbar_spin_bounded(bar, parity, abort_flag, status_word, status_code);
   return __any_sync(0xffffffffu, *abort_flag) == 0;
 }
+
+// Position in a ring of `stages` slots.
+struct RingPosition {
+  int slot = 0;
+  uint32_t parity = 0;
+  __device__ __forceinline__ void next(int stages) {
+    if (++slot == stages) {
+      slot = 0;
+      parity ^= 1u;
+    }
+  }
+};
 
 // warp_wait for a barrier on which both CTAs of a pair arrive: what the other CTA did before its arrival is
 // ordered before what follows here.
