@@ -10,7 +10,7 @@
 //   warp 0      copies of both operands' codes and scale tiles by TMA; every CTA needs the scales of all 256 rows of
 //               b.  Both CTAs' copies complete on the first CTA's barrier (the cta_group::2 form of the copy)
 //   warp 1      first CTA: scales to tensor memory (both CTAs') and MMAs
-//   warps 2-5   epilogue
+//   warps 2-9   epilogue
 //
 // Tensor memory holds two accumulators of 256 columns that overlap, [0, 256) and [208, 464), beside the 48 columns
 // of scales.  The epilogue reads the shared columns of a tile first and gives them back at once; the next
@@ -28,7 +28,7 @@ namespace {
 
 constexpr int kRowsCta = 128;   // rows of a, and of b, that one CTA loads
 constexpr int kRowsPair = 256;
-constexpr int kEpilogueWarps = 4;
+constexpr int kEpilogueWarps = 8;  // two per quarter of the lanes, a chunk of columns each in turn
 constexpr int kThreads = 32 * (2 + kEpilogueWarps);
 constexpr int kMaxStages = 6;
 constexpr int kStatusPairWait = 620;
@@ -68,8 +68,8 @@ struct PairTile {
   static constexpr int kBytesScaleA = kTiles * 512;
   static constexpr int kBytesScaleB = 2 * kTiles * 512;
   static constexpr int kStageBytes = 2 * kBytesCodes + kBytesScaleA + kBytesScaleB;
-  static constexpr int kStages = (kSmemLimit - 2048 - kEpilogueWarps * kStagingBytes) / kStageBytes < kMaxStages
-                                     ? (kSmemLimit - 2048 - kEpilogueWarps * kStagingBytes) / kStageBytes
+  static constexpr int kStages = (kSmemLimit - 1280 - kEpilogueWarps * kStagingBytes) / kStageBytes < kMaxStages
+                                     ? (kSmemLimit - 1280 - kEpilogueWarps * kStagingBytes) / kStageBytes
                                      : kMaxStages;
   static constexpr int kSmemBytes = kStages * kStageBytes + kEpilogueWarps * kStagingBytes + 1024;
   static_assert(kTiles * 4 * 3 <= 48, "scale columns");
@@ -280,6 +280,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float alpha = product_factor(p.factor_a, p.factor_b);
     const uint32_t acc_free = map_to_cta(smem_addr(&bars.acc_free), leader);
     const int quarter = warp & 3;
+    const int group = (warp - 2) >> 2;
     uint8_t* mine = staging + (warp - 2) * kStagingBytes;
     int n = 0;
     for (int t = first_tile; t < tiles; t += tile_step, ++n) {
@@ -291,14 +292,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after_sync();
       const uint32_t acc = tmem + (n & 1) * kSecondAccumulator + (static_cast<uint32_t>(quarter * 32) << 16);
 #pragma unroll 1
-      for (int c = 0; c < kRowsPair / kChunk; ++c) {
+      for (int c = group; c < kRowsPair / kChunk; c += kEpilogueWarps / 4) {
         // The columns shared with the other accumulator come first: the last ones of [0, 256), the first of [208, 464).
         const int first_col = ((n & 1) ? c : kRowsPair / kChunk - 1 - c) * kChunk;
         uint32_t v[2][32];
         tmem_load_32cols(acc + first_col, v[0]);
         tmem_load_32cols(acc + first_col + 32, v[1]);
         tmem_load_wait();
-        if (c == 0) {
+        if (c == group) {  // the shared columns have been read, or this warp has no part in them: tile n - 1 is done
           tc_fence_before_sync();
           __syncwarp();
           if (lane == 0) arrive_remote(acc_free);
@@ -311,6 +312,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if constexpr (kSplit) {
     constexpr int kOwnChunks = kRowsPair / kChunk / 2;  // a pair stores half of the columns
     const int quarter = warp & 3;
+    const int group = (warp - 2) >> 2;
     const uint32_t acc = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     bool ok = false;
     if (warp >= 2) {
@@ -324,7 +326,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t place = smem_addr(smem) + static_cast<uint32_t>(quarter * 32 + lane) * 4;
     if (ok) {
 #pragma unroll 1
-      for (int c = 0; c < kOwnChunks; ++c) {
+      for (int c = group; c < kOwnChunks; c += kEpilogueWarps / 4) {
         const int column = ((1 - slice) * kOwnChunks + c) * kChunk;
         const uint32_t to = map_to_cta(place + static_cast<uint32_t>(c) * (kChunk * kRowsCta * 4), in_cluster ^ 2u);
         uint32_t v[2][32];
@@ -345,7 +347,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tile_of(p, first_tile, &tile_a, &tile_b);
       const int row0 = tile_a * kRowsPair + static_cast<int>(rank) * kRowsCta + quarter * 32;
 #pragma unroll 1
-      for (int c = 0; c < kOwnChunks; ++c) {
+      for (int c = group; c < kOwnChunks; c += kEpilogueWarps / 4) {
         const int column = (slice * kOwnChunks + c) * kChunk;
         uint32_t v[2][32];
         tmem_load_32cols(acc + column, v[0]);

@@ -165,9 +165,24 @@ struct RingPosition {
 // ordered before what follows here.
 __device__ __forceinline__ bool warp_wait_pair(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
                                                int* status_word, int status_code) {
-  const bool ok = warp_wait(bar, parity, abort_flag, status_word, status_code);
-  asm volatile("fence.acq_rel.cluster;" ::: "memory");
-  return ok;
+  const long long start = clock64();
+  while (true) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(smem_addr(bar)), "r"(parity)
+        : "memory");
+    if (__all_sync(0xffffffffu, done != 0)) return true;
+    const bool late = clock64() - start > kWaitLimitCycles;
+    if (late) {
+      *abort_flag = 1;
+      atomicCAS(status_word, 0, status_code);
+    }
+    if (__any_sync(0xffffffffu, late || *abort_flag != 0)) return false;
+  }
 }
 
 // One lane of a converged warp.  The warps that issue copies and MMAs run their loops with all lanes and
