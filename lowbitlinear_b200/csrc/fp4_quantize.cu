@@ -5,11 +5,12 @@
 //   dequantise  x = code * step, one rounding to the output type
 //
 // Both are bound by HBM: a value is read (or written) once in 2 or 4 bytes, and 0.53 (MXFP4) or 0.56
-// (NVFP4) bytes per value go the other way.  A thread owns sixteen neighbouring columns: one NVFP4
-// block, or half of an MXFP4 block whose other half sits in the neighbouring lane, so the largest
-// magnitude takes at most one shuffle; four scale bytes meet by shuffles and leave as one word.  Rows are read and
-// written in 32-byte pieces per lane; rows that do not start on 16 bytes go through shared memory, where a warp
-// turns its 512 neighbouring columns from "a lane, one column after the other" to sixteen per lane.
+// (NVFP4) bytes per value go the other way.  A thread owns sixteen neighbouring columns; the quantiser of a large
+// matrix of a 16-bit type 32, so that what a thread does besides its values (addresses, steps, scale words)
+// weighs less: at two bytes per value the instructions are as scarce as the bandwidth (24576 x 4096 FP16 to NVFP4
+// 49.4 us with sixteen, 42.7 with 32; 333 x 1003 2.0 and 2.8).  The largest magnitude of a block takes at most one
+// shuffle; four scale bytes meet by shuffles and leave as one word.  Rows are read and written in 32-byte pieces per lane; rows that do not start on 16 bytes go through shared
+// memory, where a warp turns its columns from "a lane, one column after the other" to sixteen per lane.
 #include "fp4_common.cuh"
 #include "kernels.h"
 
@@ -17,64 +18,89 @@ namespace lbl {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kWarpCols = 512;  // columns of a row that one warp handles
+constexpr int kWarpUnits = 32 * 16;  // columns of a row that one warp handles, per sixteen of a thread
 
-// One thread per (row, sixteen columns); rows are padded to whole scale tiles, so that every byte of
+// One thread per (row, 16 kUnits columns); rows are padded to whole scale tiles, so that every byte of
 // the scale buffer is written (zero where there is no value).
-template <typename T, int kFormat>
+template <typename T, int kFormat, int kUnits>
 __global__ void __launch_bounds__(kThreads)
     fp4_quantize_kernel(const T* __restrict__ x, int64_t row_stride, const float* __restrict__ factor,
                         uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int rows, int cols, int pitch,
                         int tiles, int access, bool early_successor) {
   pdl_wait_for_previous_kernel();
   if (early_successor) pdl_allow_next_kernel();
+  constexpr int kWarpCols = kWarpUnits * kUnits;
   const int lane = threadIdx.x & 31;
   const int row = blockIdx.y * blockDim.y + threadIdx.y;  // of this launch: fewer than 65536
-  const int unit = blockIdx.x * blockDim.x + threadIdx.x;  // blockDim.x is a multiple of 32: a warp has one row
+  const int thread = blockIdx.x * blockDim.x + threadIdx.x;  // blockDim.x is a multiple of 32: a warp has one row
   if (row >= ((rows + 127) & ~127)) return;
-  const int first = unit * 16;
-  const int valid = row < rows ? min(16, cols - first) : 0;  // columns to read; below zero past the last one
+  const int first = thread * (16 * kUnits);
+  const int left = row < rows ? cols - first : 0;  // columns to read; below zero past the last one
 
-  fp4::Sixteen<T> v;
+  fp4::Sixteen<T> v[kUnits];
   const T* src = x + (row * row_stride + first);
   if (access == fp4::kRowsAny) {
     extern __shared__ __align__(32) uint8_t turned[];
     T* mine = reinterpret_cast<T*>(turned) + (threadIdx.y * blockDim.x + threadIdx.x) / 32 * kWarpCols;
-    const T* line = src - lane * 16;
-    const int end = row < rows ? cols - first + lane * 16 : 0;
+    const T* line = src - lane * (16 * kUnits);
+    const int end = row < rows ? cols - first + lane * (16 * kUnits) : 0;
 #pragma unroll
     for (int i = 0; i < kWarpCols / 32; ++i) {
       const int c = i * 32 + lane;
       mine[c] = c < end ? line[c] : static_cast<T>(0.0f);
     }
     __syncwarp();
-    v.load_vector(mine + lane * 16, fp4::kRows16);
-  } else if (valid == 16) {
-    v.load_vector(src, access);
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) v[u].load_vector(mine + (lane * kUnits + u) * 16, fp4::kRows16);
   } else {
-    v.load_masked(src, valid);
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      if (left >= 16 * (u + 1)) {
+        v[u].load_vector(src + 16 * u, access);
+      } else {
+        v[u].load_masked(src + 16 * u, left - 16 * u);
+      }
+    }
   }
-  uint32_t amax = v.amax_bits();
-  fp4::BlockStep step;
-  if constexpr (kFormat == fp4::kMx) {
-    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    step = fp4::mx_step(amax);
-  } else {
-    step = fp4::nv_step(amax, fp4::tensor_factor(factor));
-  }
-  const uint2 out = fp4::round_sixteen<kFormat>(v, step);
-  const bool stored = row < rows && unit * 8 < pitch;
-  if (stored) *reinterpret_cast<uint2*>(codes + static_cast<int64_t>(row) * pitch + unit * 8) = out;
 
-  // Blocks with no column (padding of the last tile, padding rows) have scale zero.
-  uint32_t byte = stored ? step.byte : 0u;
-  constexpr int kSpan = kFormat == fp4::kMx ? 2 : 1;  // lanes per block
-  const int place = (lane / kSpan) & 3;
-  uint32_t word = byte << (8 * place);
-  word |= __shfl_xor_sync(0xffffffffu, word, kSpan);
-  word |= __shfl_xor_sync(0xffffffffu, word, 2 * kSpan);
-  const int tile = unit / (4 * kSpan);
-  if (lane % (4 * kSpan) == 0 && tile < tiles) {
+  // Bytes of this thread's blocks, at their place in the word of four; blocks with no column (padding of the last tile,
+  // padding rows) have scale zero.
+  constexpr int kLanesPerWord = 8 / kUnits / (kFormat == fp4::kNv ? 2 : 1);
+  const bool stored = row < rows && first < 2 * pitch;
+  uint32_t word = 0;
+  uint2 out[kUnits];
+  if constexpr (kFormat == fp4::kMx) {
+    uint32_t amax = v[0].amax_bits();
+    if constexpr (kUnits == 2) {
+      amax = max(amax, v[1].amax_bits());
+    } else {
+      amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    }
+    const fp4::BlockStep step = fp4::mx_step(amax);
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) out[u] = fp4::round_sixteen<kFormat>(v[u], step);
+    if (stored) word = step.byte << (8 * (lane * kUnits / 2 & 3));
+  } else {
+    const fp4::TensorFactor g = fp4::tensor_factor(factor);
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      const fp4::BlockStep step = fp4::nv_step(v[u].amax_bits(), g);
+      out[u] = fp4::round_sixteen<kFormat>(v[u], step);
+      if (stored) word |= step.byte << (8 * (lane * kUnits + u & 3));
+    }
+  }
+  if (stored) {
+    uint8_t* dst = codes + (static_cast<int64_t>(row) * pitch + first / 2);
+    if constexpr (kUnits == 2) {
+      *reinterpret_cast<uint4*>(dst) = make_uint4(out[0].x, out[0].y, out[1].x, out[1].y);
+    } else {
+      *reinterpret_cast<uint2*>(dst) = out[0];
+    }
+  }
+#pragma unroll
+  for (int offset = kLanesPerWord / 2; offset > 0; offset >>= 1) word |= __shfl_xor_sync(0xffffffffu, word, offset);
+  const int tile = thread / kLanesPerWord;
+  if (lane % kLanesPerWord == 0 && tile < tiles) {
     *reinterpret_cast<uint32_t*>(scales + fp4::scale_word_offset(row, tile, tiles)) = word;
   }
 }
@@ -128,7 +154,7 @@ __global__ void __launch_bounds__(kThreads)
   T* dst = out + (static_cast<int64_t>(row) * cols + first);
   if (access == fp4::kRowsAny) {
     extern __shared__ __align__(32) uint8_t turned[];
-    T* mine = reinterpret_cast<T*>(turned) + (threadIdx.y * blockDim.x + threadIdx.x) / 32 * kWarpCols;
+    T* mine = reinterpret_cast<T*>(turned) + (threadIdx.y * blockDim.x + threadIdx.x) / 32 * kWarpUnits;
     if (first < cols) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) mine[lane * 16 + i] = static_cast<T>(v[i]);
@@ -137,7 +163,7 @@ __global__ void __launch_bounds__(kThreads)
     T* line = dst - lane * 16;
     const int end = cols - first + lane * 16;
 #pragma unroll
-    for (int i = 0; i < kWarpCols / 32; ++i) {
+    for (int i = 0; i < kWarpUnits / 32; ++i) {
       const int c = i * 32 + lane;
       if (c < end) line[c] = mine[c];
     }
@@ -169,12 +195,15 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
-// blockDim = (32 * columns of warps, rows): short rows share a CTA.
-dim3 block_for(int64_t units) {
-  const int64_t warps = (units + 31) / 32;
-  int x = 1;
-  while (x < 8 && x < warps) x *= 2;
-  return dim3(32 * x, kThreads / (32 * x));
+// blockDim = (32 * warps along a row, rows): eight warps, of which as many work along a row as leave the fewest idle
+// in its last CTA.
+dim3 block_for(int64_t threads) {
+  const int64_t warps = (threads + 31) / 32;
+  int best = 1;
+  for (int x = 2; x <= 8 && x <= warps; x *= 2) {
+    if ((warps + x - 1) / x * x <= (warps + best - 1) / best * best) best = x;
+  }
+  return dim3(32 * best, kThreads / (32 * best));
 }
 
 constexpr int64_t kRowsPerLaunch = 65535 / 128 * 128;  // limit of the grid's y extent, in whole scale tiles
@@ -193,47 +222,61 @@ cudaError_t launch(void (*kernel)(Parameters...), dim3 grid, dim3 block, size_t 
   return cudaLaunchKernelEx(&cfg, kernel, Parameters(arguments)...);
 }
 
-template <typename T, int kFormat>
-cudaError_t quantize(const void* x, int64_t row_stride, const float* factor, uint8_t* codes, uint8_t* scales,
-                     int64_t rows, int64_t cols, bool early_successor, cudaStream_t stream) {
+template <typename T, int kFormat, int kUnits>
+cudaError_t quantize_units(const void* x, int64_t row_stride, const float* factor, uint8_t* codes, uint8_t* scales,
+                           int64_t rows, int64_t cols, bool early_successor, cudaStream_t stream) {
   const int64_t tiles = fp4::scale_tiles(cols, kFormat);
-  const int64_t units = tiles * fp4::Format<kFormat>::kTileCols / 16;
-  const dim3 block = block_for(units);
-  const int64_t blocks_x = (units + block.x - 1) / block.x;
+  const int64_t pitch = fp4::code_pitch(cols);
+  const int64_t threads = tiles * fp4::Format<kFormat>::kTileCols / (16 * kUnits);
+  const dim3 block = block_for(threads);
+  const int64_t blocks_x = (threads + block.x - 1) / block.x;
   const int64_t padded = (rows + 127) / 128 * 128;
   if (blocks_x > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
   const int access = fp4::row_access(x, row_stride * static_cast<int64_t>(sizeof(T)));
-  const size_t smem = access == fp4::kRowsAny ? kThreads / 32 * kWarpCols * sizeof(T) : 0;
+  const size_t smem = access == fp4::kRowsAny ? kThreads / 32 * kWarpUnits * kUnits * sizeof(T) : 0;
   for (int64_t r0 = 0; r0 < padded; r0 += kRowsPerLaunch) {
     const int64_t here = rows - r0 < kRowsPerLaunch ? rows - r0 : kRowsPerLaunch;
     const int64_t here_padded = (here + 127) / 128 * 128;
     const dim3 grid(static_cast<unsigned>(blocks_x), static_cast<unsigned>((here_padded + block.y - 1) / block.y));
     const cudaError_t err = launch(
-        fp4_quantize_kernel<T, kFormat>, grid, block, smem, stream, static_cast<const T*>(x) + r0 * row_stride, row_stride, factor, codes + r0 * fp4::code_pitch(cols),
-        scales + r0 / 128 * tiles * 512, static_cast<int>(here), static_cast<int>(cols),
-        static_cast<int>(fp4::code_pitch(cols)), static_cast<int>(tiles), access, early_successor);
+        fp4_quantize_kernel<T, kFormat, kUnits>, grid, block, smem, stream, static_cast<const T*>(x) + r0 * row_stride,
+        row_stride, factor, codes + r0 * pitch, scales + r0 / 128 * tiles * 512, here, cols, pitch, tiles, access,
+        early_successor);
     if (err != cudaSuccess) return err;
   }
   return cudaSuccess;
 }
 
 template <typename T, int kFormat>
+cudaError_t quantize(const void* x, int64_t row_stride, const float* factor, uint8_t* codes, uint8_t* scales,
+                     int64_t rows, int64_t cols, bool early_successor, cudaStream_t stream) {
+  // 32 columns per thread once that still fills a B200 twice with threads; rows that go through shared memory keep
+  // sixteen (20000 x 1003 to MXFP4 14.0 us, 15.6 with 32).
+  if constexpr (sizeof(T) == 2) {
+    if (rows * cols >= 2LL * 148 * 2048 * 32 && fp4::row_access(x, row_stride * 2) != fp4::kRowsAny) {
+      return quantize_units<T, kFormat, 2>(x, row_stride, factor, codes, scales, rows, cols, early_successor, stream);
+    }
+  }
+  return quantize_units<T, kFormat, 1>(x, row_stride, factor, codes, scales, rows, cols, early_successor, stream);
+}
+
+template <typename T, int kFormat>
 cudaError_t dequantize(const uint8_t* codes, const uint8_t* scales, const float* factor, void* out, int64_t rows,
                        int64_t cols, cudaStream_t stream) {
   const int64_t tiles = fp4::scale_tiles(cols, kFormat);
+  const int64_t pitch = fp4::code_pitch(cols);
   const int64_t units = (cols + 15) / 16;
   const dim3 block = block_for(units);
   const int64_t blocks_x = (units + block.x - 1) / block.x;
   if (blocks_x > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
   const int access = fp4::row_access(out, cols * static_cast<int64_t>(sizeof(T)));
-  const size_t smem = access == fp4::kRowsAny ? kThreads / 32 * kWarpCols * sizeof(T) : 0;
+  const size_t smem = access == fp4::kRowsAny ? kThreads / 32 * kWarpUnits * sizeof(T) : 0;
   for (int64_t r0 = 0; r0 < rows; r0 += kRowsPerLaunch) {
     const int64_t here = rows - r0 < kRowsPerLaunch ? rows - r0 : kRowsPerLaunch;
     const dim3 grid(static_cast<unsigned>(blocks_x), static_cast<unsigned>((here + block.y - 1) / block.y));
     const cudaError_t err = launch(
-        fp4_dequantize_kernel<T, kFormat>, grid, block, smem, stream, codes + r0 * fp4::code_pitch(cols), scales + r0 / 128 * tiles * 512, factor, static_cast<T*>(out) + r0 * cols,
-        static_cast<int>(here), static_cast<int>(cols), static_cast<int>(fp4::code_pitch(cols)), static_cast<int>(tiles),
-        access);
+        fp4_dequantize_kernel<T, kFormat>, grid, block, smem, stream, codes + r0 * pitch, scales + r0 / 128 * tiles * 512,
+        factor, static_cast<T*>(out) + r0 * cols, here, cols, pitch, tiles, access);
     if (err != cudaSuccess) return err;
   }
   return cudaSuccess;

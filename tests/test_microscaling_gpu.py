@@ -106,6 +106,24 @@ def test_more_rows_than_one_grid_holds(cuda_ops, fmt):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("rows,cols", [(2500, 8000), (1301, 15368), (9000, 2200)])
+def test_large_matrices_get_the_codes_of_small_ones(cuda_ops, fmt, dtype, rows, cols):
+    """Large matrices take more columns per thread: same codes and scales as block after block of 128 rows, and
+    the oracle's for some of the rows."""
+    x = hard_values(64, cols, dtype, cols).to(cuda_ops).repeat(rows // 64 + 1, 1)[:rows].contiguous()
+    x[1::3] = torch.randn(x[1::3].shape, device=cuda_ops).to(dtype)
+    g = on(cuda_ops, factor_of(fmt, 2.0**-6))
+    codes, scales = quantize_fp4(x, fmt, g)
+    for r0 in range(0, rows, 128):
+        small = quantize_fp4(x[r0:r0 + 128], fmt, g)
+        assert torch.equal(codes[r0:r0 + 128], small[0]) and torch.equal(scales[r0 // 128], small[1][0])
+    picked = [0, 1, 2, 63, 130, rows - 1]
+    want, _ = oracle.quantize(x[picked].double().cpu().numpy(), fmt, item(g))
+    assert np.array_equal(codes[picked].cpu().numpy(), oracle.pack(want))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 128, 64), (1, 129, 32), (2, 127, 33), (8, 64, 31), (9, 300, 96), (16, 256, 128),
                                    (17, 513, 160), (32, 130, 256), (33, 128, 257), (64, 200, 1000), (65, 77, 288),
                                    (128, 256, 512), (129, 255, 320), (256, 512, 1024), (300, 1030, 900), (520, 520, 4096)])
