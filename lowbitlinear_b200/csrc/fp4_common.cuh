@@ -55,7 +55,6 @@ __device__ __forceinline__ float e4m3_to_float(uint32_t byte) {
 struct BlockStep {
   uint32_t byte;  // scale as stored
   float step, mul, mul_low;
-  float limit;  // NVFP4: eight steps when the scale has saturated, infinity otherwise
   bool short_step;  // NVFP4: the step has the four bits of an E4M3 number (g is a power of two)
 };
 
@@ -83,7 +82,7 @@ __device__ __forceinline__ BlockStep mx_step(uint32_t amax_bits) {
   const bool bad = exponent == 255u;
   b.byte = bad ? 0xFFu : byte;
   b.mul = bad ? 0.0f : __uint_as_float((254u - byte) << 23);
-  b.step = 0.0f, b.mul_low = 0.0f, b.limit = 0.0f, b.short_step = false;  // not used
+  b.step = 0.0f, b.mul_low = 0.0f, b.short_step = false;  // not used
   return b;
 }
 
@@ -114,7 +113,6 @@ __device__ __forceinline__ BlockStep nv_step(uint32_t amax_bits, const TensorFac
   b.mul = none ? 0.0f : __fdividef(1.0f - 0x1p-21f, b.step);
   b.mul_low = none ? 0.0f : fmaf(-b.mul, b.step, 1.0f) * b.mul;
   b.short_step = f.power_of_two;
-  b.limit = byte >= 0x7Eu ? 8.0f * b.step : __uint_as_float(0x7F800000u);
   return b;
 }
 
@@ -132,31 +130,57 @@ __device__ __forceinline__ uint32_t eight_codes(const float (&q)[8]) {
   return out;
 }
 
+// NVFP4 quotients of eight values, to 40 bits and rounded once; both products have the sign of x, zeros included.
+// kSettled: a number of at most eleven bits over a step of four is either on a border (at most seven bits: three
+// of the border, four of the step), and then comes out as the border itself, or at least 2^-11 of it away.
+// Otherwise the rounding may have put a quotient on a border that it only comes near to.  Borders have three bits;
+// when one of the quotients has no more (a zero, or one in 2^20), the sign of its exact remainder decides, and one
+// unit in the last place moves it to its side.
+template <bool kSettled>
+__device__ __forceinline__ void nv_quotients(const float (&x)[8], const BlockStep& b, float (&q)[8]) {
+  uint32_t lowest = 0xFFFFFFFFu;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    q[i] = fmaf(x[i], b.mul, x[i] * b.mul_low);
+    if (!kSettled) lowest = min(lowest, __float_as_uint(q[i]) << 11);
+  }
+  if (!kSettled && lowest == 0) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float size = fabsf(q[i]);
+      const float remainder = fmaf(-size, b.step, fabsf(x[i]));
+      const int move = (remainder > 0.0f ? 1 : 0) - (remainder < 0.0f ? 1 : 0);
+      const bool border = (__float_as_uint(size) << 11) == 0 && size < 8.0f;  // beyond, everything becomes 6
+      if (border) q[i] = copysignf(__int_as_float(__float_as_int(size) + move), x[i]);
+    }
+  }
+}
+
 // Codes of sixteen neighbouring values (Sixteen<T> below).
 template <int kFormat, typename Values>
 __device__ __forceinline__ uint2 round_sixteen(const Values& v, const BlockStep& b) {
   uint32_t codes[2];
   float x[8], q[8];
-  if (kFormat == kMx || (Values::kHalf && b.short_step)) {
+  if constexpr (kFormat == kMx) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       v.eight(h, x);
-      // NVFP4: the quotient to 40 bits, rounded once.  A number of at most eleven bits is either on a border (at most
-      // seven bits: three of the code's border, four of the step), and then comes out as the border itself, or at
-      // least 2^-11 of it away.  Both products have the sign of x, zeros included.
 #pragma unroll
-      for (int i = 0; i < 8; ++i) q[i] = kFormat == kMx ? x[i] * b.mul : fmaf(x[i], b.mul, x[i] * b.mul_low);
+      for (int i = 0; i < 8; ++i) q[i] = x[i] * b.mul;  // exact
+      codes[h] = eight_codes(q);
+    }
+  } else if (Values::kHalf && b.short_step) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      v.eight(h, x);
+      nv_quotients<true>(x, b, q);
       codes[h] = eight_codes(q);
     }
   } else {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       v.eight(h, x);
-      // Only a saturated scale (8 steps < amax) makes the bound finite.  The sign of a zero is kept.
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        q[i] = copysignf(sided_quotient(fminf(fabsf(x[i]), b.limit), b.step, b.mul), x[i]);
-      }
+      nv_quotients<false>(x, b, q);
       codes[h] = eight_codes(q);
     }
   }

@@ -5,6 +5,8 @@
     python -m lowbitlinear_b200.profile --operator gemm  --shape 16x4096x4096 --path gemm_tc_small
     python -m lowbitlinear_b200.profile --operator group --layers 2 --launches 3
     python -m lowbitlinear_b200.profile --operator quantize --shape 1x8192x4096 --launches 3
+    python -m lowbitlinear_b200.profile --operator fp4_linear --shape 2048x8192x4096 --format nvfp4 --launches 3
+    python -m lowbitlinear_b200.profile --operator fp4_quantize --shape 1x8192x4096 --format mxfp4 --launches 3
     torchrun --nproc-per-node 2 -m lowbitlinear_b200.profile --operator exchange_trace --layers 36
 
 Plays the role of the reference's ``benchmarks/profile_w4a16.py``: inputs are prepared and the
@@ -13,7 +15,8 @@ times, cycling through ``--copies`` distinct copies of the weights (so that a de
 HBM rather than the L2).  ``--path`` forces one kernel of the dispatcher (generic, gemv,
 gemv_splitk, gemm_tc, gemm_tc_small); ``--operator group`` runs the grouped decode launch over
 ``--layers`` Qwen3-8B-shaped layers (four linears each, 120 MB of weights per layer);
-``--operator quantize`` runs the device quantiser on an FP16 weight of the given N x K.
+``--operator quantize`` runs the device quantiser on an FP16 weight of the given N x K;
+``--operator fp4_linear`` and ``fp4_quantize`` run the microscaled FP4 layer (BF16 activations) and quantiser.
 ``--operator exchange_trace`` (one process per GPU under torchrun; library built with
 ``python -m lowbitlinear_b200.build --force -D LBL_TRACE_EXCHANGE``) replays the tensor-parallel
 decode step of ``--layers`` layers and prints, per replay, the %globaltimer stamps that the grouped
@@ -108,7 +111,9 @@ def exchange_trace(args):
 
 def main(argv=None):
     parser = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
-    parser.add_argument("--operator", choices=("gemv", "gemm", "group", "quantize", "exchange_trace"), required=True)
+    parser.add_argument("--operator", choices=("gemv", "gemm", "group", "quantize", "fp4_linear", "fp4_quantize", "exchange_trace"),
+                        required=True)
+    parser.add_argument("--format", choices=("mxfp4", "nvfp4"), default="mxfp4", help="of the fp4 operators")
     parser.add_argument("--shape", default=None, help="MxNxK")
     parser.add_argument("--path", choices=tuple(v for v in _ops.PATH_NAMES.values() if v != "auto"), default=None)
     parser.add_argument("--layers", type=int, default=2)
@@ -158,6 +163,31 @@ def main(argv=None):
             packed, scales, zeros = _ops.quantize_pack(weight)
         torch.cuda.synchronize()
         print(f"PASS quantize shape={n}x{k} launches={args.launches} bit-exact on 256 rows; no latency is reported here")
+        return
+
+    if args.operator.startswith("fp4"):
+        from .microscaling import MicroscaledLinear, dequantize_fp4, quantize_fp4
+        weight = (torch.randn(n, k, device=device, generator=g) * 0.02).bfloat16()
+        layer = MicroscaledLinear.from_float(weight, args.format)
+        if args.operator == "fp4_quantize":
+            codes, scales = quantize_fp4(weight[:256].cpu(), args.format,
+                                         None if layer.tensor_scale is None else layer.tensor_scale.cpu())
+            assert torch.equal(layer.codes[:256].cpu(), codes) and torch.equal(layer.scales[:2].cpu(), scales[:2])
+            for _ in range(args.launches):
+                quantize_fp4(weight, args.format, layer.tensor_scale)
+        else:
+            x = torch.randn(m, k, device=device, generator=g).bfloat16()
+            values = [dequantize_fp4(c, s, k, args.format, f, torch.float32)
+                      for c, s, f in ((*quantize_fp4(x, args.format), None), (layer.codes, layer.scales, layer.tensor_scale))]
+            rel = rel_l2(layer(x), values[0] @ values[1].T)
+            assert rel <= 4e-3, f"relative L2 error {rel:.3e}"  # one rounding to BF16
+            layers = [layer] + [MicroscaledLinear(layer.codes.clone(), layer.scales.clone(), layer.tensor_scale,
+                                                  in_features=k, format=args.format) for _ in range(args.copies - 1)]
+            for i in range(args.launches):
+                layers[i % len(layers)](x)
+        torch.cuda.synchronize()
+        print(f"PASS {args.operator} shape={m}x{n}x{k} format={args.format} launches={args.launches}; "
+              "no latency is reported here")
         return
 
     x = torch.randn(m, k, device=device, generator=g).half()

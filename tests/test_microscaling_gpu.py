@@ -62,6 +62,35 @@ def test_quantize_and_dequantize_match_the_oracle(cuda_ops, fmt, dtype, factor, 
         assert torch.equal(got.cpu(), want.float().to(out))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_values_next_to_the_borders_fall_on_the_right_side(cuda_ops, dtype):
+    """NVFP4 values on a border between two codes and one or two units in the last place beside it, for tensor
+    factors that are powers of two and others; for the 16-bit types the factor is moved instead, since their
+    own numbers are too coarse to come that near."""
+    rng = np.random.default_rng(11)
+    borders = np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0])
+    scales = oracle.E4M3[rng.integers(40, 120, 60)]
+    if dtype == torch.float32:
+        factors = [2.0**-6, 0.0123, 1 / 3, 7.1e-5]
+    else:
+        grid = torch.tensor([1.0009765625, 1.37, 1.9, 2.0**-3 * 1.21]).to(dtype).double().numpy()
+        factors = [float(np.float32(x / (b * s)) + np.float32(k) * np.spacing(np.float32(x / (b * s))))
+                   for x in grid for b, s in ((1.25, 13.0), (3.5, 0.6875), (0.75, 28.0)) for k in (-1, 0, 1)]
+    for factor in factors:
+        g = np.float32(factor)
+        step = (scales.astype(np.float32) * g).astype(np.float32)
+        near = (step[:, None].astype(np.float64) * borders).astype(np.float32)
+        rows = [near]
+        for _ in range(2):
+            rows += [np.nextafter(rows[-1], np.float32(np.inf)), np.nextafter(near, np.float32(0))]
+        x = np.concatenate([np.concatenate([(6 * step)[:, None], r, -r, np.zeros((len(step), 1), np.float32)], 1) for r in rows])
+        x = torch.from_numpy(x).to(dtype)
+        codes, got_scales = quantize_fp4(x.to(cuda_ops), "nvfp4", torch.tensor([factor], device=cuda_ops))
+        want_codes, want_bytes = oracle.quantize(x.double().numpy(), "nvfp4", factor)
+        assert np.array_equal(got_scales.cpu().numpy(), oracle.tile(want_bytes))
+        assert np.array_equal(codes.cpu().numpy(), oracle.pack(want_codes))
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("dtype", TYPES)
 def test_values_that_are_not_finite_and_extremes(cuda_ops, fmt, dtype):
