@@ -48,7 +48,7 @@ struct PairParams {
   int rows_a, rows_b;
   int cols_padded;
   int tiles_a, tiles_b;
-  int vector_ok;  // 16-byte stores of out allowed
+  int vector_ok;  // rows of out start on 16 bytes
   int* status;
 };
 
@@ -119,7 +119,8 @@ __device__ __forceinline__ void tile_of(const PairParams& p, int t, int* tile_a,
 }
 
 // One warp's 32 rows x 64 columns of sums, a row per lane, to out through the warp's staging memory, so that rows leave
-// as whole 128-byte runs.
+// as whole 128-byte runs: eight lanes per row in 16-byte pieces where rows of out start on 16 bytes, and
+// otherwise a row per store, in 4-byte words that start on a word (one column later on rows that do not).
 template <typename T>
 __device__ __forceinline__ void store_chunk(const PairParams& p, const uint32_t (&v)[2][32], float alpha,
                                             uint8_t* staging, int row0, int col0, int lane) {
@@ -136,25 +137,31 @@ __device__ __forceinline__ void store_chunk(const PairParams& p, const uint32_t 
   }
   __syncwarp();
   T* out = static_cast<T*>(p.out);
-  const int piece = lane & 7;
-  const int col = col0 + piece * 8;
+  if (p.vector_ok) {  // rows_b is a multiple of eight then
+    const int piece = lane & 7;
+    const int col = col0 + piece * 8;
 #pragma unroll
-  for (int r = lane >> 3; r < 32; r += 4) {
-    const uint4 q = *reinterpret_cast<const uint4*>(staging + r * 128 + ((piece ^ (r & 7)) << 4));
-    const int row = row0 + r;
-    if (row < p.rows_a && col < p.rows_b) {
-      T* dst = out + row * p.out_pitch + col;
-      if (p.vector_ok && col + 8 <= p.rows_b) {
-        *reinterpret_cast<uint4*>(dst) = q;
-      } else {
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (col + e < p.rows_b) {
-            reinterpret_cast<unsigned short*>(dst)[e] = static_cast<unsigned short>(w[e >> 1] >> (16 * (e & 1)));
-          }
-        }
+    for (int r = lane >> 3; r < 32; r += 4) {
+      const uint4 q = *reinterpret_cast<const uint4*>(staging + r * 128 + ((piece ^ (r & 7)) << 4));
+      if (row0 + r < p.rows_a && col < p.rows_b) *reinterpret_cast<uint4*>(out + (row0 + r) * p.out_pitch + col) = q;
+    }
+  } else {
+    const int columns = min(kChunk, p.rows_b - col0);
+    const int rows = min(32, p.rows_a - row0);
+#pragma unroll 4
+    for (int r = 0; r < rows; ++r) {
+      unsigned short* line = reinterpret_cast<unsigned short*>(out + (row0 + r) * p.out_pitch + col0);
+      auto value = [&](int c) {
+        return *reinterpret_cast<const unsigned short*>(staging + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2);
+      };
+      const int late = static_cast<int>(reinterpret_cast<uintptr_t>(line) >> 1) & 1;
+      const int c = 2 * lane + late;
+      if (c + 1 < columns) {
+        *reinterpret_cast<uint32_t*>(line + c) = value(c) | (static_cast<uint32_t>(value(c + 1)) << 16);
+      } else if (c < columns) {
+        line[c] = value(c);
       }
+      if (late && lane == 0 && columns > 0) line[0] = value(0);
     }
   }
   __syncwarp();

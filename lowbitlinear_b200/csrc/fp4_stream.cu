@@ -36,6 +36,7 @@ struct StreamParams {
   int cols;         // K
   int cols_padded;  // to 32
   int scale_tiles;  // along K
+  int out_words;    // rows of out start on eight bytes
   int stages;
   int split;        // CTAs of a cluster, a power of two
   int split_shift;  // its logarithm
@@ -65,7 +66,7 @@ struct StreamTile {
   static constexpr int kPartialBytes = kP * kQ * 4;
   static constexpr int kColumns = kQ + kTiles * 4 * (1 + kQBlocks);
   static constexpr int kTmemColumns = kColumns <= 64 ? 64 : kColumns <= 128 ? 128 : kColumns <= 256 ? 256 : 512;
-  static constexpr int kWorkers = kFused ? 8 : 4;  // warps
+  static constexpr int kWorkers = 8;  // warps
   static constexpr int kThreads = 32 * (2 + kWorkers);
 };
 
@@ -253,11 +254,12 @@ __global__ void __launch_bounds__(StreamTile<kFormat, kQ, kFused>::kThreads, 2)
   // Row q of the tile is summed by CTA q % split, which receives [slice][q / split][128] FP32.
   const int slots = kQ >> p.split_shift;
   uint8_t* received = smem + p.receive_offset;
-  if (warp >= 2 && warp < 6) {
+  if (warp >= 2) {
+    // Two warps per quarter of the lanes, 32 columns in turn.
     const int quarter = warp & 3;
     const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     const uint32_t mine = smem_addr(received) + (rank * slots * kP + quarter * 32 + lane) * 4;
-    for (int c0 = 0; c0 < used; c0 += 32) {
+    for (int c0 = ((warp - 2) >> 2) * 32; c0 < used; c0 += 64) {
       uint32_t v[32];
       tmem_load_32cols(taddr + c0, v);
       tmem_load_wait();
@@ -290,30 +292,31 @@ __global__ void __launch_bounds__(StreamTile<kFormat, kQ, kFused>::kThreads, 2)
     tmem_dealloc(tmem, Tile::kTmemColumns);
   }
 
-  // Two neighbouring rows of the weight and one activation row per thread and step; slices in their order.
+  // Four neighbouring rows of the weight and one activation row per thread and step; slices in their order.
   const float alpha = product_factor(p.factor_p, p.factor_q);
   T* out = static_cast<T*>(p.out);
-  const bool paired = (p.out_pitch & 1) == 0 && (reinterpret_cast<uintptr_t>(out) & 3) == 0;
   const int my_rows = used > static_cast<int>(rank) ? (used - static_cast<int>(rank) + p.split - 1) >> p.split_shift : 0;
-  for (int item = threadIdx.x; item < my_rows * (kP / 2); item += Tile::kThreads) {
-    const int slot = item / (kP / 2);
-    const int row = (item % (kP / 2)) * 2;
-    const int q = (slot << p.split_shift) + rank;
-    const float2* part = reinterpret_cast<const float2*>(received) + (slot * kP + row) / 2;
-    float a = 0.0f, b = 0.0f;
+  const int stride = slots * (kP / 4);
 #pragma unroll 4
-    for (int r = 0; r < p.split; ++r) {
-      const float2 v = part[r * slots * (kP / 2)];
-      a += v.x, b += v.y;
+  for (int item = threadIdx.x; item < my_rows * (kP / 4); item += Tile::kThreads) {
+    const int slot = item / (kP / 4);
+    const int row = (item % (kP / 4)) * 4;
+    const float4* part = reinterpret_cast<const float4*>(received) + item;
+    float4 sum = part[0];
+    for (int r = 1; r < p.split; ++r) {
+      const float4 v = part[r * stride];
+      sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
     }
-    if (p0 + row >= p.rows_p) continue;
-    T* dst = out + (q0 + q) * p.out_pitch + p0 + row;
-    const uint32_t y = two_rounded<T>(a * alpha, b * alpha);
-    if (paired && p0 + row + 1 < p.rows_p) {
-      *reinterpret_cast<uint32_t*>(dst) = y;
+    const int left = p.rows_p - (p0 + row);
+    T* dst = out + (q0 + (slot << p.split_shift) + rank) * p.out_pitch + p0 + row;
+    const uint32_t y[2] = {two_rounded<T>(sum.x * alpha, sum.y * alpha), two_rounded<T>(sum.z * alpha, sum.w * alpha)};
+    if (p.out_words && left >= 4) {
+      *reinterpret_cast<uint2*>(dst) = make_uint2(y[0], y[1]);
     } else {
-      *reinterpret_cast<unsigned short*>(dst) = static_cast<unsigned short>(y & 0xFFFFu);
-      if (p0 + row + 1 < p.rows_p) *(reinterpret_cast<unsigned short*>(dst) + 1) = static_cast<unsigned short>(y >> 16);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i < left) reinterpret_cast<unsigned short*>(dst)[i] = static_cast<unsigned short>(y[i >> 1] >> (16 * (i & 1)));
+      }
     }
   }
 }
@@ -371,6 +374,7 @@ cudaError_t launch(const Fp4Operand& w, const Fp4Operand& x, const void* raw, in
   params.cols = static_cast<int>(K);
   params.cols_padded = static_cast<int>(fp4::padded_cols(K));
   params.scale_tiles = static_cast<int>(fp4::scale_tiles(K, kFormat));
+  params.out_words = w.rows % 4 == 0 && reinterpret_cast<uintptr_t>(out) % 8 == 0;
   params.split = split;
   params.split_shift = 0;
   while ((1 << params.split_shift) < split) ++params.split_shift;
