@@ -48,7 +48,7 @@ struct PairParams {
   int rows_a, rows_b;
   int cols_padded;
   int tiles_a, tiles_b;
-  int vector_ok;  // rows of out start on 16 bytes
+  int out_bytes;  // rows of out start on 16 or 8 bytes, or anywhere (2)
   int* status;
 };
 
@@ -119,8 +119,8 @@ __device__ __forceinline__ void tile_of(const PairParams& p, int t, int* tile_a,
 }
 
 // One warp's 32 rows x 64 columns of sums, a row per lane, to out through the warp's staging memory, so that rows leave
-// as whole 128-byte runs: eight lanes per row in 16-byte pieces where rows of out start on 16 bytes, and
-// otherwise a row per store, in 4-byte words that start on a word (one column later on rows that do not).
+// as whole 128-byte runs: in 16- or 8-byte pieces where rows of out start on those, and otherwise a row per store, in
+// 4-byte words that start on a word (one column later on rows that do not).
 template <typename T>
 __device__ __forceinline__ void store_chunk(const PairParams& p, const uint32_t (&v)[2][32], float alpha,
                                             uint8_t* staging, int row0, int col0, int lane) {
@@ -137,7 +137,7 @@ __device__ __forceinline__ void store_chunk(const PairParams& p, const uint32_t 
   }
   __syncwarp();
   T* out = static_cast<T*>(p.out);
-  if (p.vector_ok) {  // rows_b is a multiple of eight then
+  if (p.out_bytes == 16) {  // rows_b is a multiple of eight then
     const int piece = lane & 7;
     const int col = col0 + piece * 8;
 #pragma unroll
@@ -145,23 +145,34 @@ __device__ __forceinline__ void store_chunk(const PairParams& p, const uint32_t 
       const uint4 q = *reinterpret_cast<const uint4*>(staging + r * 128 + ((piece ^ (r & 7)) << 4));
       if (row0 + r < p.rows_a && col < p.rows_b) *reinterpret_cast<uint4*>(out + (row0 + r) * p.out_pitch + col) = q;
     }
+  } else if (p.out_bytes == 8) {  // of four
+    const int piece = lane & 15;
+    const int col = col0 + piece * 4;
+#pragma unroll
+    for (int r = lane >> 4; r < 32; r += 2) {
+      const uint2 q = *reinterpret_cast<const uint2*>(staging + r * 128 + (((piece >> 1) ^ (r & 7)) << 4) + (piece & 1) * 8);
+      if (row0 + r < p.rows_a && col < p.rows_b) *reinterpret_cast<uint2*>(out + (row0 + r) * p.out_pitch + col) = q;
+    }
   } else {
     const int columns = min(kChunk, p.rows_b - col0);
-    const int rows = min(32, p.rows_a - row0);
-#pragma unroll 4
-    for (int r = 0; r < rows; ++r) {
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r) {
+      if (row0 + r >= p.rows_a) break;
       unsigned short* line = reinterpret_cast<unsigned short*>(out + (row0 + r) * p.out_pitch + col0);
-      auto value = [&](int c) {
-        return *reinterpret_cast<const unsigned short*>(staging + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2);
-      };
+      auto place = [&](int c) { return staging + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2; };
       const int late = static_cast<int>(reinterpret_cast<uintptr_t>(line) >> 1) & 1;
+      // The word of columns 2 lane and 2 lane + 1; one column later the upper half joins the next lane's lower one.
+      uint32_t word = *reinterpret_cast<const uint32_t*>(place(2 * lane));
       const int c = 2 * lane + late;
-      if (c + 1 < columns) {
-        *reinterpret_cast<uint32_t*>(line + c) = value(c) | (static_cast<uint32_t>(value(c + 1)) << 16);
+      const uint32_t next = __shfl_down_sync(0xffffffffu, word, 1);
+      const uint32_t first = word;
+      if (late) word = __funnelshift_r(word, next, 16);
+      if (c + 1 < columns && !(late && lane == 31)) {
+        *reinterpret_cast<uint32_t*>(line + c) = word;
       } else if (c < columns) {
-        line[c] = value(c);
+        line[c] = static_cast<unsigned short>(word & 0xFFFFu);
       }
-      if (late && lane == 0 && columns > 0) line[0] = value(0);
+      if (late && lane == 0 && columns > 0) line[0] = static_cast<unsigned short>(first & 0xFFFFu);
     }
   }
   __syncwarp();
@@ -420,7 +431,8 @@ cudaError_t launch(const Fp4Operand& a, const Fp4Operand& b, void* out, int64_t 
   if (tiles_a * tiles_b > 0x3fffffffLL) return cudaErrorInvalidConfiguration;
   params.tiles_a = static_cast<int>(tiles_a);
   params.tiles_b = static_cast<int>(tiles_b);
-  params.vector_ok = b.rows % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  const uintptr_t out_bits = reinterpret_cast<uintptr_t>(out) | static_cast<uintptr_t>(b.rows * sizeof(T));
+  params.out_bytes = out_bits % 16 == 0 ? 16 : out_bits % 8 == 0 ? 8 : 2;
   params.status = status;
 
   auto kernel = fp4_pair_kernel<kFormat, kSplit, T>;
