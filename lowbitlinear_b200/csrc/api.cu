@@ -453,9 +453,9 @@ size_t fp4_scale_bytes(int64_t rows, int64_t K, int format) {
 }
 
 // Which product kernel.  The pair kernel's 256 x 256 tiles from 129 rows on, when there is one for every seven SMs
-// (measured, us, streaming / pair kernel: 128 x 24576 x 4096 22.2 / 22.5, 192 rows 31 / 22.7; 128 x 6144 x 4096
-// 11.1 / 11.2, 192 rows 15.0 / 11.1; 256 x 4096 x 4096, 16 tiles, 11.4 / 12.5, 384 rows, 32 tiles, 15.0 / 11.3;
-// 256 x 4096 x 12288 17 / 27, 384 rows 25 / 18).
+// (measured, us, streaming / pair kernel: 128 x 24576 x 4096 15.7 / 18.5, 192 rows 25.6 / 18.6; 128 x 6144 x 4096
+// 9.4 / 9.5, 192 rows 10.5 / 9.6; 256 x 4096 x 4096, 16 tiles, 8.2 / 8.8, 384 rows, 32 tiles, 10.7 / 10.0;
+// 256 x 4096 x 12288 13.5 / 14.1, 384 rows 18.3 / 15.4).
 bool fp4_use_pair(int64_t M, int64_t N, int sm_count) {
   const int64_t tiles = ((M + 255) / 256) * ((N + 255) / 256);
   return M > 128 && 7 * tiles >= sm_count;

@@ -2,10 +2,11 @@
 //
 //   out[i, j] = T( ga gb sum_k a[i, k] b[j, k] )
 //
-// Bound by the tensor pipe (a pair's MMA of 256 x 256 x 64 takes 128 cycles at the FP4 rate) and by the L2,
-// which has to deliver 64 bytes per cycle and SM at that rate with 256 x 256 tiles.  A cluster of two CTAs owns a
-// tile: each loads its 128 rows of a and its half of the 256 rows of b, tcgen05.mma.cta_group::2 reads both
-// halves of b, and each CTA accumulates its 128 rows x 256 columns.
+// Bound by the tensor pipe (a pair's MMA of 256 x 256 x 64 takes 128 cycles at the FP4 rate), by the shared memory that
+// the copies write and the MMAs and scale copies read (36-39 KB and about as much per stage of 512 MMA cycles), and on
+// long runs by the power cap: 6.0 PFLOP/s on 4096 x 9472 x 16384, 5.2 on 8192 x 24576 x 4096 in short runs and 4.7 at the
+// cap.  A cluster of two CTAs owns a tile: each loads its 128 rows of a and its half of the 256 rows of b,
+// tcgen05.mma.cta_group::2 reads both halves of b, and each CTA accumulates its 128 rows x 256 columns.
 //
 //   warp 0      copies of both operands' codes and scale tiles by TMA; every CTA needs the scales of all 256 rows of
 //               b.  Both CTAs' copies complete on the first CTA's barrier (the cta_group::2 form of the copy)
@@ -16,11 +17,11 @@
 // of scales.  The epilogue reads the shared columns of a tile first and gives them back at once; the next
 // tile's MMAs start then and run beside the rest of the epilogue.
 //
-// kSplit: fewer tiles than half the pairs of SMs.  One SM takes in 45 bytes per cycle, so a tile on its own needs 7 us
-// for 4096 columns of K; two pairs of a cluster share it then, each with half of K, push the FP32 sums of the columns
-// they do not own to the pair that does (distributed shared memory, over the ring that has been read), and both
-// pairs add and store their columns, always in the same order.  (256 x 6144 x 4096: 11.5 us, 13.4 without.  Four
-// pairs, clusters of eight CTAs with 200 KB each, took 20 us: too few of them fit on the chip at once.)
+// kSplit: fewer tiles than half the pairs of SMs.  A tile on its own needs 700 cycles per stage of K; two pairs of a
+// cluster share it then, each with half of K, push the FP32 sums of the columns they do not own to the pair that does
+// (distributed shared memory, over the ring that has been read), and both pairs add and store their columns, always in
+// the same order.  (256 x 6144 x 4096 in two halves 11.5 us, 13.4 without.  Four pairs, clusters of eight CTAs
+// with 200 KB each, took 20 us: too few of them fit on the chip at once.)
 #include "fp4_tc.cuh"
 
 namespace lbl {

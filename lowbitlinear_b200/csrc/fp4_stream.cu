@@ -323,18 +323,22 @@ __global__ void __launch_bounds__(StreamTile<kFormat, kQ, kFused>::kThreads, 2)
 
 constexpr int kSmemLimit = 226 * 1024;     // dynamic shared memory of a CTA
 constexpr int kSmemPerSm = 228 * 1024;
+constexpr int kStaticSmem = (sizeof(StreamBarriers) + 127) / 128 * 128;
 constexpr int kFusedRows = 16;
-constexpr int kFusedUnits = 512;  // of sixteen columns: what the quantising warps of a CTA round in two steps
 constexpr int kRingStages = 6;
 
-// Slices of K, each on a CTA of its own: doubled until most SMs have one, and beyond that while a slice keeps four
-// stages (a second CTA on an SM hides the first one's start, but the sums cost more to join).  Measured, us, 1 / 2 /
-// 4 / 8 slices: 32 row blocks of 16 stages 8.9 / 7.1 / 5.5 / 5.8, of 48 stages 23 / 14 / 9.3 / 8.5; 48 blocks of 16
-// stages 12.6 / 9.7 / 8.2 / 10.2; 192 blocks of 16 stages 14.5 / 14.2 / 16.7 / 20.7.
-int choose_split(int64_t tiles, int k_stages, int sm_count) {
+// Slices of K, each on a CTA of its own: doubled while the CTAs still fit the SMs once and a slice keeps two stages
+// (four with more than 32 activation rows, whose sums cost more to join), and once more, to two CTAs on some SMs, while
+// it keeps six (eight).  Measured, us, 1 / 2 / 4 / 8 slices: 1 row, 32 row blocks of 16 stages 6.2 / 5.5 / 4.3 / 4.4,
+// of 48 stages 13.8 / 9.3 / 6.7 / 6.5; 32 rows, 48 blocks of 16 stages 7.5 / 6.5 / 9.8 / 9.5; 64 rows, 32 blocks of 16
+// stages 7.3 / 6.8 / 5.6 / 6.6; 77 rows, 40 blocks of 4 stages 5.1 / 5.6 / 6.3 / 6.3; 100 rows, 64 blocks of 32 stages
+// 17.3 / 13.8 / 12.4 / 20.7; 16 rows, 192 blocks of 16 stages 13.7 / 17.2 / 20.6 / 29.9.
+int choose_split(int64_t tiles, int k_stages, int tile_rows, int sm_count) {
+  const int least = tile_rows <= 32 ? 2 : 4;  // stages of a slice
+  const int least_beyond = tile_rows <= 32 ? 6 : 8;
   int split = 1;
-  while (split < kMaxSplit && k_stages >= 2 * split &&
-         (5 * tiles * split < 4 * sm_count || (tiles * split < sm_count && k_stages >= 8 * split))) {
+  while (split < kMaxSplit && ((k_stages >= 2 * split * least && 2 * tiles * split <= sm_count) ||
+                               (k_stages >= 2 * split * least_beyond && tiles * split < sm_count))) {
     split *= 2;
   }
   return split;
@@ -357,7 +361,7 @@ cudaError_t launch(const Fp4Operand& w, const Fp4Operand& x, const void* raw, in
   const int64_t blocks_p = (w.rows + kP - 1) / kP;
   const int64_t blocks_q = (x.rows + kQ - 1) / kQ;
   const int k_stages = stages_of(K);
-  const int split = choose_split(blocks_p * blocks_q, k_stages, sm_count);
+  const int split = choose_split(blocks_p * blocks_q, k_stages, kQ, sm_count);
   const int slice = (k_stages + split - 1) / split;
 
   StreamParams params;
@@ -387,7 +391,7 @@ cudaError_t launch(const Fp4Operand& w, const Fp4Operand& x, const void* raw, in
   // its pipeline cold.  At least two on an SM in any case, for the next kernel of the stream.
   const int64_t ctas = blocks_p * blocks_q * split;
   const int64_t per_sm = ctas <= 2 * sm_count ? 2 : ctas <= 3 * sm_count ? 3 : 4;
-  const int budget = static_cast<int>(kSmemPerSm / per_sm) - 1024;  // the driver takes 1 KB of each CTA's share
+  const int budget = static_cast<int>(kSmemPerSm / per_sm) - 1024 - kStaticSmem;  // the driver takes 1 KB of each CTA's share
   int stages = slice < kRingStages ? slice : kRingStages;
   while (stages > 2 && fixed + stages * Tile::kStageBytes > budget) --stages;
   params.stages = stages;
@@ -448,12 +452,18 @@ cudaError_t launch_fp4_stream(const Fp4Operand& a, const Fp4Operand& b, int form
                                : stream_product<fp4::kMx, __half>(a, b, out, K, sm_count, status_word, early_weight, stream);
 }
 
-// Every CTA rounds its slice of the activations itself: worth a launch while that is a step or two.
+// Every CTA rounds its slice of the activations itself: worth a launch while that is four rounds of the quantising warps
+// (three where CTAs share an SM) and the slice leaves the ring its depth.  Measured, us, one launch / two, NVFP4: 4096 x 4096
+// (slices of 4 stages, 128 CTAs) 1 row 4.5 / 6.9, 8 rows 5.6 / 6.9, 16 rows 6.9 / 7.0; 6144 x 4096 (8, 96 CTAs) 8 rows
+// 7.8 / 7.6, 12 rows 8.8 / 7.7; 8192 x 8192 (8, 256 CTAs) 1 row 9.4 / 12.5, 6 rows 11.2 / 12.5, 12 rows 13.5 / 12.5;
+// 5120 x 12288 (12, 160 CTAs) 1 row 9.7 / 12.2, 6 rows 12.8 / 12.2; 24576 x 4096 (16, 192 CTAs) 1 row 14.7 / 13.9.
 bool fp4_fused_supports(int64_t M, int64_t N, int64_t K, int sm_count) {
   if (M > kFusedRows) return false;
   const int64_t k_stages = stages_of(K);
-  const int split = choose_split((N + kP - 1) / kP, static_cast<int>(k_stages), sm_count);
-  return M * 16 * ((k_stages + split - 1) / split) <= kFusedUnits;
+  const int64_t blocks = (N + kP - 1) / kP;
+  const int split = choose_split(blocks, static_cast<int>(k_stages), kFusedRows, sm_count);
+  const int64_t slice = (k_stages + split - 1) / split;
+  return blocks * split <= sm_count ? slice <= 16 && M * slice <= 64 : slice <= 12 && M * slice <= 48;
 }
 
 cudaError_t launch_fp4_fused_linear(const void* x, int x_type, int64_t x_stride, int64_t M, const float* x_factor,
