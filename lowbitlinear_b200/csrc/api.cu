@@ -545,7 +545,7 @@ int lbl_fp4_matmul(const void* a_codes, const void* a_scales, const float* a_fac
 
 size_t lbl_fp4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int format) {
   if (M <= 0 || N <= 0 || K <= 0 || (format != LBL_FP4_MX && format != LBL_FP4_NV)) return 0;
-  if (lbl::fp4_fused_supports(M, N, K, sm_count_or_default(-1))) return 0;
+  if (lbl::fp4_fused_supports(M, N, K, format, sm_count_or_default(-1))) return 0;
   return fp4_code_bytes(M, K) + fp4_scale_bytes(M, K, format);
 }
 

@@ -453,17 +453,19 @@ cudaError_t launch_fp4_stream(const Fp4Operand& a, const Fp4Operand& b, int form
 }
 
 // Every CTA rounds its slice of the activations itself: worth a launch while that is four rounds of the quantising warps
-// (three where CTAs share an SM) and the slice leaves the ring its depth.  Measured, us, one launch / two, NVFP4: 4096 x 4096
-// (slices of 4 stages, 128 CTAs) 1 row 4.5 / 6.9, 8 rows 5.6 / 6.9, 16 rows 6.9 / 7.0; 6144 x 4096 (8, 96 CTAs) 8 rows
-// 7.8 / 7.6, 12 rows 8.8 / 7.7; 8192 x 8192 (8, 256 CTAs) 1 row 9.4 / 12.5, 6 rows 11.2 / 12.5, 12 rows 13.5 / 12.5;
-// 5120 x 12288 (12, 160 CTAs) 1 row 9.7 / 12.2, 6 rows 12.8 / 12.2; 24576 x 4096 (16, 192 CTAs) 1 row 14.7 / 13.9.
-bool fp4_fused_supports(int64_t M, int64_t N, int64_t K, int sm_count) {
+// (three where CTAs share an SM) and the slice leaves three stages to the ring.  Measured, us, one launch / two, NVFP4:
+// 4096 x 4096 (slices of 4 stages, 128 CTAs) 1 row 4.5 / 6.9, 8 rows 5.6 / 6.9, 16 rows 6.9 / 7.0; 6144 x 4096 (8, 96
+// CTAs) 8 rows 7.8 / 7.6, 12 rows 8.8 / 7.7; 8192 x 8192 (8, 256 CTAs) 1 row 9.4 / 12.5, 6 rows 11.2 / 12.5, 12 rows 13.5
+// / 12.5; 5120 x 12288 (12, 160 CTAs) 1 row 9.7 / 12.2, 6 rows 12.8 / 12.2; 24576 x 4096 (16, 192 CTAs; two stages left)
+// 1 row 14.7 / 13.9, in MXFP4 (smaller scale tiles, three stages) 11.7 / 13.2.
+bool fp4_fused_supports(int64_t M, int64_t N, int64_t K, int format, int sm_count) {
   if (M > kFusedRows) return false;
   const int64_t k_stages = stages_of(K);
   const int64_t blocks = (N + kP - 1) / kP;
   const int split = choose_split(blocks, static_cast<int>(k_stages), kFusedRows, sm_count);
   const int64_t slice = (k_stages + split - 1) / split;
-  return blocks * split <= sm_count ? slice <= 16 && M * slice <= 64 : slice <= 12 && M * slice <= 48;
+  if (blocks * split <= sm_count) return slice <= 16 && M * slice <= 64;
+  return slice <= (format == fp4::kNv ? 12 : 16) && M * slice <= 48;
 }
 
 cudaError_t launch_fp4_fused_linear(const void* x, int x_type, int64_t x_stride, int64_t M, const float* x_factor,

@@ -193,7 +193,7 @@ struct Fp4Operand {
 cudaError_t launch_fp4_stream(const Fp4Operand& a, const Fp4Operand& b, int format, void* out, int out_type, int64_t K,
                               int sm_count, int* status_word, bool early_weight, cudaStream_t stream);
 // The same with a given as 16-bit activations x [M, K], quantised in the kernel; out has their type.
-bool fp4_fused_supports(int64_t M, int64_t N, int64_t K, int sm_count);
+bool fp4_fused_supports(int64_t M, int64_t N, int64_t K, int format, int sm_count);
 cudaError_t launch_fp4_fused_linear(const void* x, int x_type, int64_t x_stride, int64_t M, const float* x_factor,
                                     const Fp4Operand& w, int format, void* out, int64_t K, int sm_count,
                                     int* status_word, bool early_weight, cudaStream_t stream);

@@ -177,6 +177,27 @@ def test_large_products_match_64_bits(cuda_ops, fmt, m, n, k):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+def test_offsets_past_32_bits(cuda_ops, fmt):
+    """Matrices and products of more than 2^31 elements: their last rows are what the same rows are alone."""
+    rows, cols = 66001, 33000
+    tail = hard_values(300, cols, torch.bfloat16, 1).to(cuda_ops)
+    x = torch.zeros(rows, cols, dtype=torch.bfloat16, device=cuda_ops)
+    x[-300:] = tail
+    codes, scales = quantize_fp4(x, fmt)
+    want = quantize_fp4(tail, fmt)
+    assert torch.equal(codes[-300:], want[0]) and not codes[:-300].any()
+    y = dequantize_fp4(codes, scales, cols, fmt, dtype=torch.bfloat16)
+    assert torch.equal(y[-300:], dequantize_fp4(*want, cols, fmt, dtype=torch.bfloat16)) and not y[:-300].any()
+    del x, y, codes, scales
+    a = quantize_fp4(torch.randn(rows, 96, device=cuda_ops), fmt)
+    b = quantize_fp4(torch.randn(cols, 96, device=cuda_ops), fmt)
+    got = matmul_fp4(*a, *b, fmt)
+    values = [dequantize_fp4(*t, 96, fmt, dtype=torch.float32).double().cpu().numpy() for t in (a, b)]
+    for r in (slice(0, 2), slice(65534, 65538), slice(rows - 2, rows)):
+        check_product(got[r], values[0][r], values[1], torch.float16)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("m", [1, 3, 16, 40, 200, 600, 3000])
 def test_rows_do_not_touch_each_other(cuda_ops, fmt, m):
     """A row whose blocks are NaN makes its own outputs NaN; an all-zero row gives zeros; every other
@@ -213,6 +234,25 @@ def test_linear_matches_64_bits(cuda_ops, fmt, dtype, m, n, k):
     got = linear_fp4(x.to(cuda_ops), wc.to(cuda_ops), ws.to(cuda_ops), fmt, on(cuda_ops, factor_of(fmt, wf)), on(cuda_ops, g))
     assert got.dtype == dtype
     check_product(got, oracle.values(xc, xb, fmt, item(g)), w, dtype)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("m,n,k", [(1, 9601, 4000), (4, 9601, 4000), (5, 9601, 4000), (6, 8200, 8100), (7, 8200, 8100), (4, 5000, 12201),
+                                   (3, 20001, 1500), (16, 33001, 500), (12, 2049, 8191)])
+def test_wide_layers_with_few_rows_match_64_bits(cuda_ops, fmt, m, n, k):
+    """Few rows on wide weights: one CTA per SM or several, long slices of K and short ones, and row counts on
+    both sides of where the activations are quantised by a launch of their own."""
+    g = torch.Generator(cuda_ops).manual_seed(m + n)
+    weight = quantize_fp4(torch.randn(n, k, device=cuda_ops, generator=g).half(), fmt)
+    x = hard_values(m, k, torch.bfloat16, m + n).clamp(-500, 500)
+    got = linear_fp4(x.to(cuda_ops), *weight, fmt)
+    xc, xb = oracle.quantize(x.double().numpy(), fmt)
+    a = oracle.values(xc, xb, fmt)
+    padded = a.shape[1]
+    b = dequantize_fp4(*weight, padded, fmt, dtype=torch.float32)
+    columns = torch.cat((torch.arange(0, n, 11), torch.arange(n - 130, n))).to(cuda_ops)
+    check_product(got[:, columns], a, b[columns].double().cpu().numpy(), torch.bfloat16)
+    assert torch.equal(got, matmul_fp4(*quantize_fp4(x.to(cuda_ops), fmt), *weight, fmt, dtype=torch.bfloat16))
 
 
 @pytest.mark.parametrize("m", [1, 5, 40, 300])
