@@ -176,6 +176,17 @@ def test_large_products_match_64_bits(cuda_ops, fmt, m, n, k):
     test_product_matches_64_bits(cuda_ops, fmt, m, n, k)
 
 
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("n", [257, 258, 259, 260, 319, 321, 322, 323, 328, 511])
+def test_rows_of_any_alignment_leave_the_large_product(cuda_ops, dtype, n):
+    """Outputs whose rows start on a word or not, with the last columns in every place of a store."""
+    m, k = 3001, 64
+    ac, as_, a = stored(m, k, "mxfp4", n)
+    bc, bs, b = stored(n, k, "mxfp4", n + 1)
+    got = matmul_fp4(ac.to(cuda_ops), as_.to(cuda_ops), bc.to(cuda_ops), bs.to(cuda_ops), "mxfp4", dtype=dtype)
+    check_product(got, a, b, dtype)
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_offsets_past_32_bits(cuda_ops, fmt):
     """Matrices and products of more than 2^31 elements: their last rows are what the same rows are alone."""
