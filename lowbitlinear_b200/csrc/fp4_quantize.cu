@@ -9,8 +9,9 @@
 // matrix of a 16-bit type 32, so that what a thread does besides its values (addresses, steps, scale words)
 // weighs less: at two bytes per value the instructions are as scarce as the bandwidth (24576 x 4096 FP16 to NVFP4
 // 49.4 us with sixteen, 42.7 with 32; 333 x 1003 2.0 and 2.8).  The largest magnitude of a block takes at most one
-// shuffle; four scale bytes meet by shuffles and leave as one word.  Rows are read and written in 32-byte pieces per lane; rows that do not start on 16 bytes go through shared
-// memory, where a warp turns its columns from "a lane, one column after the other" to sixteen per lane.
+// shuffle; four scale bytes meet by shuffles and leave as one word.  Rows are read and written in 32-byte pieces
+// per lane; rows that do not start on 16 bytes go through shared memory, where a warp turns its columns from a word per
+// lane to sixteen columns per lane (24576 x 4095 BF16 to NVFP4 68 us and back 59; a value at a time 69 and 63).
 #include "fp4_common.cuh"
 #include "kernels.h"
 
@@ -19,6 +20,64 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarpUnits = 32 * 16;  // columns of a row that one warp handles, per sixteen of a thread
+constexpr int kWarpWords = kWarpUnits / 2;         // of two 16-bit columns
+constexpr int kTurnedBytes = kWarpWords * 4 + 16;  // shared memory in which a warp turns them: one word more, on 16 bytes
+
+// Columns [0, end) of a row of 16-bit values that starts on any address, as eight words of two columns per lane: lane l
+// gets columns 16 l to 16 l + 15, zero past the end.  Read a word per lane, from the last word boundary at or before the
+// row's start; the value that shares a word with something else is read alone.
+__device__ __forceinline__ void load_any_row(const unsigned short* line, int end, uint8_t* turned, int lane, uint32_t (&w)[8]) {
+  uint32_t* words = reinterpret_cast<uint32_t*>(turned);
+  const int late = static_cast<int>(reinterpret_cast<uintptr_t>(line) >> 1) & 1;  // word k: columns 2 k - late, 2 k - late + 1
+  const int last = min(end, kWarpUnits) - 1;
+  uint32_t raw[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int c = 2 * (i * 32 + lane) - late;
+    raw[i] = c >= 0 && c + 1 < end ? *reinterpret_cast<const uint32_t*>(line + c) : 0u;
+  }
+  const bool single = lane == 0 ? late && end > 0 : lane == 1 && last >= 0 && ((last + late) & 1) == 0;
+  const int at = lane == 0 ? 0 : last;
+  const unsigned short value = single ? line[at] : static_cast<unsigned short>(0);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) words[i * 32 + lane] = raw[i];
+  if (lane == 0) words[kWarpWords] = 0;
+  __syncwarp();
+  if (single) reinterpret_cast<unsigned short*>(turned)[at + late] = value;
+  __syncwarp();
+  const uint4 a = *reinterpret_cast<const uint4*>(words + lane * 8);
+  const uint4 b = *reinterpret_cast<const uint4*>(words + lane * 8 + 4);
+  w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+  if (late) {
+    const uint32_t next = words[lane * 8 + 8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = __funnelshift_r(w[i], i < 7 ? w[i + 1] : next, 16);
+  }
+}
+
+// The inverse: words of columns 16 l to 16 l + 15 of lane l to columns [0, end) of such a row.
+__device__ __forceinline__ void store_any_row(unsigned short* line, int end, uint8_t* turned, int lane, const uint32_t (&w)[8]) {
+  uint32_t* words = reinterpret_cast<uint32_t*>(turned);
+  const int late = static_cast<int>(reinterpret_cast<uintptr_t>(line) >> 1) & 1;  // words start one column later
+  const int last = min(end, kWarpUnits) - 1;
+  *reinterpret_cast<uint4*>(words + lane * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+  *reinterpret_cast<uint4*>(words + lane * 8 + 4) = make_uint4(w[4], w[5], w[6], w[7]);
+  __syncwarp();
+  uint32_t raw[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int k = i * 32 + lane;
+    raw[i] = late ? __funnelshift_r(words[k], words[k + 1], 16) : words[k];
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int c = 2 * (i * 32 + lane) + late;
+    if (c + 1 <= last) *reinterpret_cast<uint32_t*>(line + c) = raw[i];
+  }
+  const bool single = lane == 0 ? late && end > 0 : lane == 1 && last >= late && ((last - late) & 1) == 0;
+  const int at = lane == 0 ? 0 : last;
+  if (single) line[at] = reinterpret_cast<const unsigned short*>(turned)[at];
+}
 
 // One thread per (row, 16 kUnits columns); rows are padded to whole scale tiles, so that every byte of
 // the scale buffer is written (zero where there is no value).
@@ -29,7 +88,6 @@ __global__ void __launch_bounds__(kThreads)
                         int tiles, int access, bool early_successor) {
   pdl_wait_for_previous_kernel();
   if (early_successor) pdl_allow_next_kernel();
-  constexpr int kWarpCols = kWarpUnits * kUnits;
   const int lane = threadIdx.x & 31;
   const int row = blockIdx.y * blockDim.y + threadIdx.y;  // of this launch: fewer than 65536
   const int thread = blockIdx.x * blockDim.x + threadIdx.x;  // blockDim.x is a multiple of 32: a warp has one row
@@ -39,19 +97,23 @@ __global__ void __launch_bounds__(kThreads)
 
   fp4::Sixteen<T> v[kUnits];
   const T* src = x + (row * row_stride + first);
-  if (access == fp4::kRowsAny) {
+  if (kUnits == 1 && access == fp4::kRowsAny) {
     extern __shared__ __align__(32) uint8_t turned[];
-    T* mine = reinterpret_cast<T*>(turned) + (threadIdx.y * blockDim.x + threadIdx.x) / 32 * kWarpCols;
-    const T* line = src - lane * (16 * kUnits);
-    const int end = row < rows ? cols - first + lane * (16 * kUnits) : 0;
+    const int warp = (threadIdx.y * blockDim.x + threadIdx.x) / 32;
+    const T* line = src - lane * 16;
+    const int end = row < rows ? cols - first + lane * 16 : 0;
+    if constexpr (sizeof(T) == 2) {
+      load_any_row(reinterpret_cast<const unsigned short*>(line), end, turned + warp * kTurnedBytes, lane, v[0].w);
+    } else {
+      T* mine = reinterpret_cast<T*>(turned) + warp * kWarpUnits;
 #pragma unroll
-    for (int i = 0; i < kWarpCols / 32; ++i) {
-      const int c = i * 32 + lane;
-      mine[c] = c < end ? line[c] : static_cast<T>(0.0f);
+      for (int i = 0; i < kWarpUnits / 32; ++i) {
+        const int c = i * 32 + lane;
+        mine[c] = c < end ? line[c] : static_cast<T>(0.0f);
+      }
+      __syncwarp();
+      v[0].load_vector(mine + lane * 16, fp4::kRows16);
     }
-    __syncwarp();
-#pragma unroll
-    for (int u = 0; u < kUnits; ++u) v[u].load_vector(mine + (lane * kUnits + u) * 16, fp4::kRows16);
   } else {
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
@@ -130,7 +192,7 @@ __global__ void __launch_bounds__(kThreads)
   const int unit = blockIdx.x * blockDim.x + threadIdx.x;  // blockDim.x is a multiple of 32: a warp has one row
   const int first = unit * 16;
   if (row >= rows) return;
-  float v[16];
+  float v[16] = {};
   if (first < cols) {
     const uint2 raw = __ldg(reinterpret_cast<const uint2*>(codes + static_cast<int64_t>(row) * pitch + unit * 8));
     constexpr int kSpan = kFormat == fp4::kMx ? 2 : 1;
@@ -154,18 +216,24 @@ __global__ void __launch_bounds__(kThreads)
   T* dst = out + (static_cast<int64_t>(row) * cols + first);
   if (access == fp4::kRowsAny) {
     extern __shared__ __align__(32) uint8_t turned[];
-    T* mine = reinterpret_cast<T*>(turned) + (threadIdx.y * blockDim.x + threadIdx.x) / 32 * kWarpUnits;
-    if (first < cols) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) mine[lane * 16 + i] = static_cast<T>(v[i]);
-    }
-    __syncwarp();
+    const int warp = (threadIdx.y * blockDim.x + threadIdx.x) / 32;
     T* line = dst - lane * 16;
     const int end = cols - first + lane * 16;
+    if constexpr (sizeof(T) == 2) {
+      uint32_t w[8];
 #pragma unroll
-    for (int i = 0; i < kWarpUnits / 32; ++i) {
-      const int c = i * 32 + lane;
-      if (c < end) line[c] = mine[c];
+      for (int i = 0; i < 8; ++i) w[i] = two_rounded<T>(v[2 * i], v[2 * i + 1]);
+      store_any_row(reinterpret_cast<unsigned short*>(line), end, turned + warp * kTurnedBytes, lane, w);
+    } else {
+      T* mine = reinterpret_cast<T*>(turned) + warp * kWarpUnits;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mine[lane * 16 + i] = v[i];
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < kWarpUnits / 32; ++i) {
+        const int c = i * 32 + lane;
+        if (c < end) line[c] = mine[c];
+      }
     }
   } else if (first + 16 <= cols) {
     uint32_t w[8];
@@ -222,6 +290,11 @@ cudaError_t launch(void (*kernel)(Parameters...), dim3 grid, dim3 block, size_t 
   return cudaLaunchKernelEx(&cfg, kernel, Parameters(arguments)...);
 }
 
+template <typename T>
+constexpr size_t turned_bytes() {
+  return kThreads / 32 * (sizeof(T) == 2 ? kTurnedBytes : kWarpUnits * sizeof(T));
+}
+
 template <typename T, int kFormat, int kUnits>
 cudaError_t quantize_units(const void* x, int64_t row_stride, const float* factor, uint8_t* codes, uint8_t* scales,
                            int64_t rows, int64_t cols, bool early_successor, cudaStream_t stream) {
@@ -233,7 +306,7 @@ cudaError_t quantize_units(const void* x, int64_t row_stride, const float* facto
   const int64_t padded = (rows + 127) / 128 * 128;
   if (blocks_x > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
   const int access = fp4::row_access(x, row_stride * static_cast<int64_t>(sizeof(T)));
-  const size_t smem = access == fp4::kRowsAny ? kThreads / 32 * kWarpUnits * kUnits * sizeof(T) : 0;
+  const size_t smem = access == fp4::kRowsAny ? turned_bytes<T>() : 0;
   for (int64_t r0 = 0; r0 < padded; r0 += kRowsPerLaunch) {
     const int64_t here = rows - r0 < kRowsPerLaunch ? rows - r0 : kRowsPerLaunch;
     const int64_t here_padded = (here + 127) / 128 * 128;
@@ -251,7 +324,7 @@ template <typename T, int kFormat>
 cudaError_t quantize(const void* x, int64_t row_stride, const float* factor, uint8_t* codes, uint8_t* scales,
                      int64_t rows, int64_t cols, bool early_successor, cudaStream_t stream) {
   // 32 columns per thread once that still fills a B200 twice with threads; rows that go through shared memory keep
-  // sixteen (20000 x 1003 to MXFP4 14.0 us, 15.6 with 32).
+  // sixteen (20000 x 1003 to MXFP4 13.0 us, in values rather than words 13.4, with 32 of them 15.6).
   if constexpr (sizeof(T) == 2) {
     if (rows * cols >= 2LL * 148 * 2048 * 32 && fp4::row_access(x, row_stride * 2) != fp4::kRowsAny) {
       return quantize_units<T, kFormat, 2>(x, row_stride, factor, codes, scales, rows, cols, early_successor, stream);
@@ -270,7 +343,7 @@ cudaError_t dequantize(const uint8_t* codes, const uint8_t* scales, const float*
   const int64_t blocks_x = (units + block.x - 1) / block.x;
   if (blocks_x > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
   const int access = fp4::row_access(out, cols * static_cast<int64_t>(sizeof(T)));
-  const size_t smem = access == fp4::kRowsAny ? kThreads / 32 * kWarpUnits * sizeof(T) : 0;
+  const size_t smem = access == fp4::kRowsAny ? turned_bytes<T>() : 0;
   for (int64_t r0 = 0; r0 < rows; r0 += kRowsPerLaunch) {
     const int64_t here = rows - r0 < kRowsPerLaunch ? rows - r0 : kRowsPerLaunch;
     const dim3 grid(static_cast<unsigned>(blocks_x), static_cast<unsigned>((here + block.y - 1) / block.y));

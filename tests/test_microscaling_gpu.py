@@ -122,6 +122,29 @@ def test_quantize_takes_strided_and_unaligned_rows(cuda_ops):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols", [1, 2, 35, 511, 512, 513, 1003, 1026])
+def test_many_rows_that_start_on_any_address(cuda_ops, fmt, dtype, cols):
+    """Enough rows that every multiprocessor works on several, one after the other: nothing of an earlier row
+    reaches the padding of a later one."""
+    rows = 4000
+    x = hard_values(64, cols, dtype, cols).repeat(rows // 64 + 1, 1)[:rows]
+    base = torch.full((rows * cols + 3,), 100.0, dtype=dtype, device=cuda_ops)
+    codes, byte = oracle.quantize(x[:64].double().numpy(), fmt)
+    packed = torch.from_numpy(oracle.pack(codes)).to(cuda_ops)
+    values = torch.from_numpy(oracle.values(codes, byte, fmt))[:, :cols].float().to(dtype)
+    byte = torch.from_numpy(byte).to(cuda_ops)
+    for start in (0, 1, 2):
+        view = base[start:start + rows * cols].view(rows, cols)
+        view.copy_(x)
+        got = quantize_fp4(view, fmt)
+        assert torch.equal(got[0], packed.repeat(rows // 64 + 1, 1)[:rows])
+        assert torch.equal(untile_scales(got[1], rows, byte.size(1)), byte.repeat(rows // 64 + 1, 1)[:rows])
+    y = dequantize_fp4(*got, cols, fmt, dtype=dtype).cpu()
+    assert torch.equal(y, values.repeat(rows // 64 + 1, 1)[:rows])
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 def test_more_rows_than_one_grid_holds(cuda_ops, fmt):
     rows, cols = 70001, 40
     x = torch.randn(rows, cols, device=cuda_ops).bfloat16()
